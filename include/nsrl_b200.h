@@ -199,6 +199,132 @@ nsrl_status nsrl_prenorm_attention_decode_block(const int16_t* x, size_t batch, 
                                                 size_t max_len, int16_t* y, void* workspace, size_t workspace_bytes,
                                                 nsrl_device_status* status, void* stream);
 
+/* ------------------------------------------------------ rotary positions --
+ * Rotary position embedding on int16 rows (no counterpart in the reference,
+ * whose models learn positions or have none).  Pair i < rotary_dim / 2 of a
+ * head, at position p, turns by the angle p * turns[i], turns[i] in units of
+ * 2^-64 turn (its sum over positions wraps at whole turns, so far positions
+ * lose nothing).  With c, s = cos, sin of the angle in Q30:
+ *   y0 = sat_i16(rhu(x0 c - x1 s, 30)),  y1 = sat_i16(rhu(x0 s + x1 c, 30)).
+ * c and s are defined in integers: with a the angle, n the nearest multiple of
+ * 2^54 (1,024 points of the circle, C and S their Q30 cos and sin, rounded to
+ * nearest) and d = a - n in (signed) units of 2^-64 turn,
+ *   r = ((d >> 22) * 1686629713) >> 32          (d in radians, Q38)
+ *   h = (((r r) >> 32) + 2^14) >> 15            (d^2 / 2, Q30)
+ *   c = C - ((256 C h + S r + 2^37) >> 38),  s = S - ((256 S h - C r + 2^37) >> 38)
+ * (>> rounds down), then, unless amplitude is 2^30, c and s become
+ * rhu(c * amplitude, 30) and rhu(s * amplitude, 30), held to +-(2^31 - 1).
+ * c and s are within 2^-27 of the angle's cosine and sine at every position.
+ * Pairs: interleaved = 0 pairs dims i and i + rotary_dim / 2, 1 pairs dims 2i
+ * and 2i + 1.  Dims rotary_dim.. of a head pass through.  The struct lives in
+ * host memory, turns in device memory. */
+typedef struct nsrl_rotary {
+  const uint64_t* turns; /* [rotary_dim / 2] */
+  size_t rotary_dim;     /* even, 2..head_dim */
+  int32_t interleaved;
+  int32_t amplitude;     /* Q30 factor of c and s, 1..2^31-1; 2^30 = 1 */
+} nsrl_rotary;
+
+/* x rows of stride ldx elements hold `heads` heads of head_dim at their start;
+ * y rows (stride ldy) get the turned heads: y == x with ldy == ldx works in
+ * place, other overlaps are not allowed.  Row r is at position positions[r]
+ * (device int32, any sign), or r % seq_len with positions NULL.  backward != 0
+ * turns the other way: the gradient of the rows from the gradient of the
+ * turned rows.  head_dim up to 1024; columns past the heads are not touched.
+ * Any alignment works; 16-byte aligned rows with head_dim and rotary_dim
+ * multiples of 16 take wide loads. */
+nsrl_status nsrl_rotary_rows(const int16_t* x, size_t rows, size_t heads, size_t head_dim, size_t ldx,
+                             const nsrl_rotary* rotary, const int32_t* positions, size_t seq_len, int backward,
+                             int16_t* y, size_t ldy, void* stream);
+
+/* ----------------------------------------------------------- 4-bit cache --
+ * A KV cache of 4-bit codes (no counterpart in the reference).  A slot holds
+ * one token's key and value of one head.  Each group of 32 dims (the whole
+ * head below 32) of a key or value has a scale and a zero point:
+ *   zero = min, scale = max(1, ceil((max - min) / 15)),
+ *   code = round half up((x - zero) / scale), one less where zero + scale * code
+ *   would pass 32767,
+ * and stands for the integers zero + scale * code (within scale / 2 of x, or
+ * within scale where the code was lowered).  head_dim 16, 64 or 256; capacity
+ * a multiple of 16; every array 16-byte aligned.  Byte i of a slot's codes
+ * holds dim 2i in its low half and 2i + 1 in its high half; a scale word is
+ * scale | zero << 16 (uint16, int16).  scores (the attention weight each slot
+ * has gathered, Q15) and positions (its token's position) may be NULL.  The
+ * struct lives in host memory, its arrays in device memory. */
+typedef struct nsrl_q4_cache {
+  uint8_t* k_codes;   /* [batch][heads][capacity][head_dim / 2] */
+  uint8_t* v_codes;
+  uint32_t* k_scales; /* [batch][heads][capacity][max(1, head_dim / 32)] */
+  uint32_t* v_scales;
+  int32_t* scores;    /* [batch][heads][capacity] or NULL */
+  int32_t* positions; /* [batch][heads][capacity] or NULL */
+  size_t batch, heads, head_dim, capacity;
+} nsrl_q4_cache;
+
+/* Quantises rows of k and v into the cache: row b * tokens + t (stride ld
+ * elements, head h at column h * head_dim) goes to slot starts[b] + t for
+ * t < counts[b] (device int32 [batch]; counts NULL = tokens).  Its score
+ * becomes 0 and its position positions[b] + t (device int32 [batch]; NULL =
+ * the slot).  Other slots stay as they were.  A sequence whose slots do not
+ * fit (starts[b] < 0, counts[b] outside 0..tokens, or past the capacity)
+ * writes nothing and rejects the call. */
+nsrl_status nsrl_q4_cache_append(const nsrl_q4_cache* cache, const int16_t* k, const int16_t* v, size_t ld,
+                                 size_t tokens, const int32_t* starts, const int32_t* counts,
+                                 const int32_t* positions, nsrl_device_status* status, void* stream);
+
+/* The values of slots starts[b] .. starts[b] + tokens - 1 (device int32
+ * [batch]; NULL = 0) as int16 [batch][heads][tokens][head_dim], the layout of
+ * the int16 decode block's caches: exactly what an appended slot stands for
+ * (hand-made scales saturate).  A sequence whose slots do not fit is not
+ * written and rejects the call. */
+nsrl_status nsrl_q4_cache_read(const nsrl_q4_cache* cache, const int32_t* starts, size_t tokens, int16_t* k,
+                               int16_t* v, nsrl_device_status* status, void* stream);
+
+/* nsrl_attention_decode over the 4-bit cache: sequence b's query (row b of q,
+ * stride ldq elements, head h at column h * head_dim) attends over the first
+ * lens[b] slots (device int32, in 1..capacity), with their dequantised values
+ * in place of int16 ones; the same logits, base-2 softmax and rounding, so on
+ * equal values the same context.  ctx: [batch][heads * head_dim].  With
+ * cache->scores, the Q15 weight of each slot is added to its score
+ * (saturating at 2^31 - 1).  Capacity at most nsrl_q4_cache_max_capacity(). */
+size_t nsrl_q4_cache_max_capacity(void);
+nsrl_status nsrl_attention_decode_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache* cache, const int32_t* lens,
+                                     int16_t* ctx, nsrl_device_status* status, void* stream);
+
+/* Cuts every (sequence, head) of more than `keep` slots to `keep`.  Slots
+ * whose position is below `sinks`, or at least next_positions[b] - recent
+ * (device int32 [batch]: the position of the sequence's next token), stay
+ * before all others; then the higher score stays (negative ones count as 0);
+ * ties go to the lower slot.  A kept slot below `keep` stays where it is; the
+ * kept slots at or past `keep` move, in order, into the slots freed below it.
+ * lens_out[b] = min(lens[b], keep); scores_out and positions_out (layout of
+ * the cache's) get the values of slots 0 .. lens_out[b] - 1, other entries
+ * stay as they were.  lens_out, scores_out and positions_out may be lens and
+ * the cache's own arrays.  Needs cache->scores and cache->positions; lens[b]
+ * outside 0..capacity leaves the sequence alone and rejects the call.
+ * keep in 1..capacity. */
+size_t nsrl_q4_cache_evict_workspace_size(const nsrl_q4_cache* cache, size_t keep);
+nsrl_status nsrl_q4_cache_evict(const nsrl_q4_cache* cache, const int32_t* lens, const int32_t* next_positions,
+                                size_t keep, size_t sinks, size_t recent, int32_t* scores_out,
+                                int32_t* positions_out, int32_t* lens_out, void* workspace, size_t workspace_bytes,
+                                nsrl_device_status* status, void* stream);
+
+/* nsrl_prenorm_attention_decode_block over the 4-bit cache, with rotary
+ * positions (rotary NULL = none): the new token of sequence b is normalised
+ * and projected, its q and k turn by positions[b] (device int32; NULL =
+ * lens[b]), its k and v enter slot lens[b] (device int32, 0..capacity - 1),
+ * and its query attends over slots 0 .. lens[b].  The caller advances lens
+ * (and positions) after every layer of the step, and evicts between steps. */
+size_t nsrl_decode_block_q4_workspace_size(size_t batch, size_t d_model, size_t heads);
+nsrl_status nsrl_prenorm_attention_decode_block_q4(const int16_t* x, size_t batch, size_t d_model, size_t heads,
+                                                   const int16_t* rms_gamma, uint64_t rms_eps,
+                                                   const nsrl_linear_params* q, const nsrl_linear_params* k,
+                                                   const nsrl_linear_params* v, const nsrl_linear_params* o,
+                                                   const nsrl_rotary* rotary, const nsrl_q4_cache* cache,
+                                                   const int32_t* lens, const int32_t* positions, int16_t* y,
+                                                   void* workspace, size_t workspace_bytes,
+                                                   nsrl_device_status* status, void* stream);
+
 /* ----------------------------------------------- training-step exchange --
  * acc[n][k] += scaled_grad[r][n] * x[r][k] for r < rows, checked i64 adds in
  * row order (zero terms skipped), *sample_count += rows: one call of the

@@ -171,6 +171,19 @@ def _i16(x: torch.Tensor) -> torch.Tensor:
     return x.contiguous()
 
 
+def _on_current_device(t: torch.Tensor, dtype, what: str):
+    """Raises unless t is a tensor of this type on the current CUDA device (the calls run on its stream)."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
+        raise NsrlError(f"{what} must be a CUDA tensor of {dtype}")
+    if t.device.index != torch.cuda.current_device():
+        raise NsrlError(f"{what} is on {t.device}, not on the current device")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor (its width where there is one row, whose stride may be anything)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+
+
 # ----------------------------------------------------------------- linear ---
 def linear_i16_i8_i16_per_channel_checked(x: torch.Tensor, lin: Linear) -> Optional[torch.Tensor]:
     """linear.rs:115-126, one call per row of x [rows, input_dim]."""

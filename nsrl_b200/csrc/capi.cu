@@ -856,6 +856,209 @@ nsrl_status nsrl_attention_decode(const int16_t* q, const int16_t* k_cache, cons
   return NSRL_OK;
 }
 
+// -------------------------------------------------------- rotary positions --
+namespace {
+nsrl_status check_rotary(const nsrl_rotary* r, size_t head_dim) {
+  if (!r || !r->turns) return shape_fail("rotary is NULL");
+  if (r->rotary_dim < 2 || r->rotary_dim % 2 != 0 || r->rotary_dim > head_dim)
+    return shape_fail("rotary_dim must be even and in 2..head_dim");
+  if (r->interleaved != 0 && r->interleaved != 1) return shape_fail("interleaved must be 0 or 1");
+  if (r->amplitude < 1) return shape_fail("the rotary amplitude must be positive");
+  return NSRL_OK;
+}
+
+bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// The cache's shape and arrays (eviction and scores check theirs on top).
+nsrl_status check_q4(const nsrl_q4_cache* c) {
+  if (!c) return shape_fail("cache is NULL");
+  if (c->head_dim != 16 && c->head_dim != 64 && c->head_dim != 256)
+    return shape_fail("the 4-bit cache takes head_dim 16, 64 or 256");
+  if (c->heads == 0 || c->capacity == 0 || c->capacity % 16 != 0)
+    return shape_fail("heads and capacity must be nonzero, capacity a multiple of 16");
+  if (c->capacity > q4_max_capacity()) return shape_fail("capacity above nsrl_q4_cache_max_capacity()");
+  if (c->heads > (1u << 20) || c->batch > (1u << 24) / c->heads)
+    return shape_fail("batch * heads must be at most 2^24");
+  if (c->batch != 0 && (!c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales))
+    return shape_fail("a cache array is NULL");
+  if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16) || !aligned(c->k_scales, 16) || !aligned(c->v_scales, 16) ||
+      !aligned(c->scores, 16) || !aligned(c->positions, 16))
+    return shape_fail("cache arrays must be 16-byte aligned");
+  return NSRL_OK;
+}
+}  // namespace
+
+nsrl_status nsrl_rotary_rows(const int16_t* x, size_t rows, size_t heads, size_t head_dim, size_t ldx,
+                             const nsrl_rotary* rotary, const int32_t* positions, size_t seq_len, int backward,
+                             int16_t* y, size_t ldy, void* stream) {
+  if (heads == 0 || head_dim < 2 || head_dim > 1024) return shape_fail("rotary: heads >= 1 and head_dim in 2..1024");
+  const nsrl_status r = check_rotary(rotary, head_dim);
+  if (r != NSRL_OK) return r;
+  if (heads > (1u << 20) || ldx < heads * head_dim || ldy < heads * head_dim)
+    return shape_fail("rotary: rows shorter than heads * head_dim");
+  if (!positions && seq_len == 0) return shape_fail("rotary: positions or seq_len");
+  if (rows == 0) return NSRL_OK;
+  if (!x || !y) return shape_fail("NULL argument");
+  if (x == y && ldx != ldy) return shape_fail("rotary: in place needs one stride");
+  if (rows >> 31) return shape_fail("rotary: rows must be below 2^31");
+  NSRL_TRY(launch_rotary(x, rows, heads, head_dim, ldx, *rotary, positions, seq_len, backward != 0, y, ldy,
+                         (cudaStream_t)stream),
+           "rotary");
+  return NSRL_OK;
+}
+
+// ------------------------------------------------------------ 4-bit cache --
+size_t nsrl_q4_cache_max_capacity(void) { return q4_max_capacity(); }
+
+nsrl_status nsrl_q4_cache_append(const nsrl_q4_cache* cache, const int16_t* k, const int16_t* v, size_t ld,
+                                 size_t tokens, const int32_t* starts, const int32_t* counts,
+                                 const int32_t* positions, nsrl_device_status* status, void* stream) {
+  const nsrl_status r = check_q4(cache);
+  if (r != NSRL_OK) return r;
+  if (ld < cache->heads * cache->head_dim) return shape_fail("append: rows shorter than heads * head_dim");
+  if (tokens > cache->capacity) return shape_fail("append: more tokens than the capacity");
+  if (cache->batch == 0 || tokens == 0) return NSRL_OK;
+  if (!k || !v || !starts || !status) return shape_fail("NULL argument");
+  NSRL_TRY(launch_q4_append(*cache, k, v, ld, tokens, starts, counts, positions, status, (cudaStream_t)stream),
+           "q4 append");
+  return NSRL_OK;
+}
+
+nsrl_status nsrl_q4_cache_read(const nsrl_q4_cache* cache, const int32_t* starts, size_t tokens, int16_t* k,
+                               int16_t* v, nsrl_device_status* status, void* stream) {
+  const nsrl_status r = check_q4(cache);
+  if (r != NSRL_OK) return r;
+  if (tokens > cache->capacity) return shape_fail("read: more tokens than the capacity");
+  if (cache->batch == 0 || tokens == 0) return NSRL_OK;
+  if (!k || !v || !status) return shape_fail("NULL argument");
+  if (!aligned(k, 16) || !aligned(v, 16)) return shape_fail("read: k and v must be 16-byte aligned");
+  NSRL_TRY(launch_q4_read(*cache, starts, tokens, k, v, status, (cudaStream_t)stream), "q4 read");
+  return NSRL_OK;
+}
+
+nsrl_status nsrl_attention_decode_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache* cache, const int32_t* lens,
+                                     int16_t* ctx, nsrl_device_status* status, void* stream) {
+  const nsrl_status r = check_q4(cache);
+  if (r != NSRL_OK) return r;
+  if (ldq < cache->heads * cache->head_dim) return shape_fail("q rows shorter than heads * head_dim");
+  if (cache->batch == 0) return NSRL_OK;
+  if (!q || !lens || !ctx || !status) return shape_fail("NULL argument");
+  NSRL_TRY(launch_attend_q4(q, ldq, *cache, lens, 0, ctx, status, (cudaStream_t)stream), "q4 decode attention");
+  return NSRL_OK;
+}
+
+size_t nsrl_q4_cache_evict_workspace_size(const nsrl_q4_cache* cache, size_t keep) {
+  if (check_q4(cache) != NSRL_OK || keep == 0 || keep > cache->capacity) return 0;
+  return q4_evict_workspace(*cache, keep);
+}
+
+nsrl_status nsrl_q4_cache_evict(const nsrl_q4_cache* cache, const int32_t* lens, const int32_t* next_positions,
+                                size_t keep, size_t sinks, size_t recent, int32_t* scores_out,
+                                int32_t* positions_out, int32_t* lens_out, void* workspace, size_t workspace_bytes,
+                                nsrl_device_status* status, void* stream) {
+  const nsrl_status r = check_q4(cache);
+  if (r != NSRL_OK) return r;
+  if (keep == 0 || keep > cache->capacity) return shape_fail("evict: keep must be in 1..capacity");
+  if (sinks > 0x7fffffffu || recent > 0x7fffffffu) return shape_fail("evict: sinks and recent must be below 2^31");
+  if (cache->batch == 0) return NSRL_OK;
+  if (!cache->scores || !cache->positions) return shape_fail("evict: the cache keeps no scores or positions");
+  if (!lens || !next_positions || !scores_out || !positions_out || !lens_out || !status)
+    return shape_fail("NULL argument");
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < q4_evict_workspace(*cache, keep))
+    return shape_fail("workspace too small or not 16-byte aligned");
+  NSRL_TRY(launch_q4_evict(*cache, lens, next_positions, keep, sinks, recent, scores_out, positions_out, lens_out,
+                           workspace, status, (cudaStream_t)stream),
+           "q4 evict");
+  return NSRL_OK;
+}
+
+size_t nsrl_decode_block_q4_workspace_size(size_t batch, size_t d_model, size_t heads) {
+  (void)heads;
+  Carver c(nullptr);
+  c.planes(batch, d_model, true);
+  c.take<int16_t>(batch * 3 * d_model);
+  c.take<int16_t>(batch * d_model);
+  c.planes(batch, d_model, true);
+  return c.off;
+}
+
+nsrl_status nsrl_prenorm_attention_decode_block_q4(const int16_t* x, size_t batch, size_t d_model, size_t heads,
+                                                   const int16_t* rms_gamma, uint64_t rms_eps,
+                                                   const nsrl_linear_params* q, const nsrl_linear_params* k,
+                                                   const nsrl_linear_params* v, const nsrl_linear_params* o,
+                                                   const nsrl_rotary* rotary, const nsrl_q4_cache* cache,
+                                                   const int32_t* lens, const int32_t* positions, int16_t* y,
+                                                   void* workspace, size_t workspace_bytes,
+                                                   nsrl_device_status* status, void* stream) {
+  nsrl_status r = validate_attention(1, d_model, heads, q, k, v, o);
+  if (r != NSRL_OK) return r;
+  r = check_q4(cache);
+  if (r != NSRL_OK) return r;
+  if (cache->batch != batch || cache->heads != heads || cache->head_dim != d_model / heads)
+    return shape_fail("the cache has another batch, heads or head_dim");
+  if (rotary) {
+    r = check_rotary(rotary, cache->head_dim);
+    if (r != NSRL_OK) return r;
+  }
+  if (batch == 0) return NSRL_OK;
+  if (!x || !y || !status || !rms_gamma || !lens) return shape_fail("NULL argument");
+  if (!workspace || workspace_bytes < nsrl_decode_block_q4_workspace_size(batch, d_model, heads))
+    return shape_fail("workspace too small");
+  cudaStream_t s = (cudaStream_t)stream;
+  const size_t d = d_model, hd = cache->head_dim;
+  Carver c(workspace);
+  Planes xn = c.planes(batch, d, true);
+  int16_t* qkv = c.take<int16_t>(batch * 3 * d);
+  int16_t* ctx16 = c.take<int16_t>(batch * d);
+  Planes ctx = c.planes(batch, d, true);
+  if (!needs_l1(d, q, k, v)) xn.l1 = nullptr;
+  if (!needs_l1(d, o)) ctx.l1 = nullptr;
+  NSRL_TRY(launch_rms_norm(x, batch, d, rms_gamma, rms_eps, nullptr, xn, status, s), "rms norm");
+  GemmArgs g{};
+  g.a_hi = xn.hi;
+  g.a_lo = xn.lo;
+  g.a_l1 = xn.l1;
+  g.lda = d;
+  g.M = batch;
+  g.K = d;
+  g.nseg = 3;
+  g.seg[0] = seg_of(q);
+  g.seg[1] = seg_of(k);
+  g.seg[2] = seg_of(v);
+  g.epi = Epi::I16;
+  g.y = qkv;
+  g.ldy = 3 * d;
+  g.st = status;
+  NSRL_TRY(launch_gemm(g, s), "qkv projection");
+  if (rotary)
+    NSRL_TRY(launch_rotary(qkv, batch, 2 * heads, hd, 3 * d, *rotary, positions ? positions : lens, 0, false, qkv,
+                           3 * d, s),
+             "rotary");
+  NSRL_TRY(launch_q4_append(*cache, qkv + d, qkv + 2 * d, 3 * d, 1, lens, nullptr, positions ? positions : lens, status,
+                            s),
+           "q4 append");
+  NSRL_TRY(launch_attend_q4(qkv, 3 * d, *cache, lens, 1, ctx16, status, s), "q4 decode attention");
+  NSRL_TRY(launch_split_planes(ctx16, batch, d, d, ctx, s), "split planes");
+  GemmArgs og{};
+  og.a_hi = ctx.hi;
+  og.a_lo = ctx.lo;
+  og.a_l1 = ctx.l1;
+  og.lda = d;
+  og.M = batch;
+  og.K = d;
+  og.nseg = 1;
+  og.seg[0] = seg_of(o);
+  og.epi = Epi::RESID;
+  og.y = y;
+  og.ldy = d;
+  og.skip = x;
+  og.ldskip = d;
+  og.sat_counter = &status->attention_saturations;
+  og.st = status;
+  NSRL_TRY(launch_gemm(og, s), "output projection");
+  return NSRL_OK;
+}
+
 // ------------------------------------------------------------- generation --
 namespace {
 // The forward of B windows of the mini transformer (softmax attention): the

@@ -270,6 +270,26 @@ cudaError_t launch_linear_attention_step(const Planes& qkv, size_t B, size_t d, 
                                          long long* key_sums, int ttt_shift, unsigned long long* delta_l1,
                                          Planes ctx, nsrl_device_status* st, cudaStream_t stream);
 
+// Rotary positions on rows of `heads` heads (rotary.cu); y == x turns in place.
+cudaError_t launch_rotary(const int16_t* x, size_t rows, size_t heads, size_t hd, size_t ldx, const nsrl_rotary& rot,
+                          const int32_t* positions, size_t seq_len, bool backward, int16_t* y, size_t ldy,
+                          cudaStream_t s);
+
+// The 4-bit cache (q4_cache.cu, decode_q4.cu), arguments as in nsrl_b200.h.
+cudaError_t launch_q4_append(const nsrl_q4_cache& c, const int16_t* k, const int16_t* v, size_t ld, size_t tokens,
+                             const int32_t* starts, const int32_t* counts, const int32_t* positions,
+                             nsrl_device_status* st, cudaStream_t s);
+cudaError_t launch_q4_read(const nsrl_q4_cache& c, const int32_t* starts, size_t tokens, int16_t* k, int16_t* v,
+                           nsrl_device_status* st, cudaStream_t s);
+size_t q4_evict_workspace(const nsrl_q4_cache& c, size_t keep);
+cudaError_t launch_q4_evict(const nsrl_q4_cache& c, const int32_t* lens, const int32_t* next, size_t keep, size_t sinks,
+                            size_t recent, int32_t* scores_out, int32_t* positions_out, int32_t* lens_out, void* ws,
+                            nsrl_device_status* st, cudaStream_t s);
+size_t q4_max_capacity();
+// Keys attended: lens[b] + len_offset.
+cudaError_t launch_attend_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache& c, const int32_t* lens, int len_offset,
+                             int16_t* ctx, nsrl_device_status* st, cudaStream_t s);
+
 void set_error(const char* fmt, ...);
 bool tma_supported();
 

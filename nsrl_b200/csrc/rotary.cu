@@ -1,0 +1,224 @@
+// Rotary positions on int16 rows, forward and backward (nsrl_rotary_rows).
+//
+// A pair (x0, x1) at position p turns by the angle a = p * turn, kept as a
+// 64-bit fraction of a turn, so the product wraps where the angle does and far
+// positions keep every bit.  cos and sin come from the nearest of 1,024 points
+// of the circle and the remaining angle d (|d| <= 2^-11 turn = 0.0031 rad):
+// cos d = 1 - d^2 / 2 within 4e-12, sin d = d within 5e-9, both below 2^-27.
+//
+// Bound by memory: 2 bytes in and 2 out per element, against about 6 integer
+// instructions; the angle work is done once per (row, pair) into shared
+// memory and read by every head.  A block takes `rows` rows so that each of
+// its 256 threads has about four items (16 dims: two 16-byte loads and
+// stores) per head sweep, and asks for its first four items before it works
+// out the angles, which hides that work behind the loads.
+#include <algorithm>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace nsrl {
+namespace {
+
+__device__ const int32_t d_quarter_lut[257] = {NSRL_QUARTER_LUT_VALUES};
+
+constexpr int THREADS = 256;
+constexpr int MAX_PAIRS = 2048;  // (row, pair) angles of a block: 16 KB of shared memory
+constexpr int ITEMS = 4;         // items a thread loads ahead
+
+struct RotArgs {
+  const int16_t* x;
+  int16_t* y;
+  long long ldx, ldy, rows;
+  const unsigned long long* turns;
+  const int32_t* positions;
+  long long seq_len;
+  int heads, hd, half, interleaved, backward, amplitude;
+  int block_rows;
+};
+
+// Q30 cosine and sine of a 2^-64 turn (the integer recipe of nsrl_b200.h).
+__device__ __forceinline__ void cos_sin_q30(unsigned long long a, int amplitude, int& c, int& s) {
+  const unsigned n = (unsigned)((a + (1ull << 53)) >> 54);  // nearest point, 0..1024 (wraps in the sum)
+  const long long d = (long long)(a - ((unsigned long long)n << 54));
+  const int i = n & 255;
+  const int lo = d_quarter_lut[i], hi = d_quarter_lut[256 - i];
+  const bool odd = n & 256, neg = n & 512;  // quadrants 1 and 3; 2 and 3
+  int S0 = odd ? hi : lo, C0 = odd ? -lo : hi;
+  if (neg) {
+    S0 = -S0;
+    C0 = -C0;
+  }
+  const int r = __mulhi((int)(d >> 22), 1686629713);
+  const int h = (__mulhi(r, r) + (1 << 14)) >> 15;
+  const long long h256 = (long long)h << 8, half = 1ll << 37;
+  long long cc = C0 - ((C0 * h256 + (long long)S0 * r + half) >> 38);
+  long long ss = S0 - ((S0 * h256 - (long long)C0 * r + half) >> 38);
+  if (amplitude != (1 << 30)) {
+    cc = (cc * amplitude + (1ll << 29)) >> 30;
+    ss = (ss * amplitude + (1ll << 29)) >> 30;
+  }
+  // |C| may pass 2^30 by one, so an amplitude near 2 may reach 2^31: held to 2^31 - 1
+  c = (int)max(-2147483647ll, min(2147483647ll, cc));
+  s = (int)max(-2147483647ll, min(2147483647ll, ss));
+}
+
+// rhu(x0 * c + x1 * s, 30), saturated; the sum stays below 2^48.
+__device__ __forceinline__ int turn(int x0, int c, int x1, int s) {
+  const long long t = (long long)x0 * c + (long long)x1 * s + (1ll << 29);
+  return sat16((int)(t >> 30));
+}
+
+// VEC: an item is 16 dims of a head (8 pairs, or 16 dims past rotary_dim),
+// two 16-byte accesses.  Otherwise an item is one pair, or one dim past rotary_dim.
+template <bool VEC>
+__global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
+  extern __shared__ __align__(16) int32_t angles[];  // c [rows][half], then s
+  int32_t* const sc = angles;
+  int32_t* const ss = angles + a.block_rows * a.half;
+  const long long row0 = (long long)blockIdx.x * a.block_rows;
+  const int rows = (int)min((long long)a.block_rows, a.rows - row0);
+  // items of a head: the pairs, then (out of place only) the dims that pass through
+  const int turning = VEC ? a.half / 8 : a.half;
+  const int passing = a.x == a.y ? 0 : (VEC ? (a.hd - 2 * a.half) / 16 : a.hd - 2 * a.half);
+  const int per_head = turning + passing, per_row = per_head * a.heads;
+  const int items = rows * per_row;
+
+  // element offsets of an item's two accesses within its row, and its first pair
+  auto place = [&](int it, int& row, int& i0, int& i1, int& pair) {
+    row = it / per_row;
+    const int in_row = it - row * per_row;
+    const int head = in_row / per_head, slot = in_row - head * per_head;
+    const int base = head * a.hd;
+    if (slot < turning) {
+      pair = VEC ? 8 * slot : slot;
+      i0 = base + (a.interleaved ? 2 * pair : pair);
+      i1 = a.interleaved ? i0 + (VEC ? 8 : 1) : i0 + a.half;
+    } else {
+      pair = -1;
+      i0 = base + 2 * a.half + (VEC ? 16 : 1) * (slot - turning);
+      i1 = i0 + (VEC ? 8 : 0);
+    }
+  };
+
+  griddep_wait();
+  griddep_launch();
+  uint4 v0[ITEMS], v1[ITEMS];
+  auto load = [&](int it, uint4& u0, uint4& u1) {
+    int row, i0, i1, pair;
+    place(it, row, i0, i1, pair);
+    const int16_t* p = a.x + (row0 + row) * a.ldx;
+    if (VEC) {
+      u0 = *reinterpret_cast<const uint4*>(p + i0);
+      u1 = *reinterpret_cast<const uint4*>(p + i1);
+    } else {
+      u0.x = (uint32_t)(uint16_t)p[i0];
+      u1.x = (uint32_t)(uint16_t)p[i1];
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int it = threadIdx.x + k * THREADS;
+    if (it < items) load(it, v0[k], v1[k]);
+  }
+  for (int i = threadIdx.x; i < rows * a.half; i += THREADS) {
+    const int row = i / a.half, pair = i - row * a.half;
+    const long long r = row0 + row;
+    const long long p = a.positions ? (long long)a.positions[r] : r % a.seq_len;
+    int c, s;
+    cos_sin_q30((unsigned long long)p * a.turns[pair], a.amplitude, c, s);
+    sc[i] = c;
+    ss[i] = a.backward ? -s : s;
+  }
+  __syncthreads();
+
+  for (int it0 = threadIdx.x; it0 < items; it0 += ITEMS * THREADS) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int it = it0 + k * THREADS;
+      if (it >= items) continue;
+      if (it0 >= ITEMS * THREADS) load(it, v0[k], v1[k]);  // past the items loaded ahead
+      int row, i0, i1, pair;
+      place(it, row, i0, i1, pair);
+      int16_t* p = a.y + (row0 + row) * a.ldy;
+      const int32_t* c = sc + row * a.half + pair;
+      const int32_t* s = ss + row * a.half + pair;
+      if (VEC) {
+        uint4 o0 = v0[k], o1 = v1[k];
+        if (pair >= 0) {
+          int e0[8], e1[8], r0[8], r1[8], cw[8], sw[8];
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            *reinterpret_cast<int4*>(cw + i) = *reinterpret_cast<const int4*>(c + i);
+            *reinterpret_cast<int4*>(sw + i) = *reinterpret_cast<const int4*>(s + i);
+          }
+          unpack8(v0[k], e0);
+          unpack8(v1[k], e1);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int x0 = a.interleaved ? (i < 4 ? e0[2 * i & 7] : e1[2 * i & 7]) : e0[i];
+            const int x1 = a.interleaved ? (i < 4 ? e0[(2 * i & 7) + 1] : e1[(2 * i & 7) + 1]) : e1[i];
+            r0[i] = turn(x0, cw[i], x1, -sw[i]);
+            r1[i] = turn(x0, sw[i], x1, cw[i]);
+          }
+          if (a.interleaved) {
+            const int m0[8] = {r0[0], r1[0], r0[1], r1[1], r0[2], r1[2], r0[3], r1[3]};
+            const int m1[8] = {r0[4], r1[4], r0[5], r1[5], r0[6], r1[6], r0[7], r1[7]};
+            o0 = pack8(m0);
+            o1 = pack8(m1);
+          } else {
+            o0 = pack8(r0);
+            o1 = pack8(r1);
+          }
+        }
+        *reinterpret_cast<uint4*>(p + i0) = o0;
+        *reinterpret_cast<uint4*>(p + i1) = o1;
+      } else {
+        const int x0 = (int)(int16_t)v0[k].x, x1 = (int)(int16_t)v1[k].x;
+        p[i0] = (int16_t)(pair >= 0 ? turn(x0, c[0], x1, -s[0]) : x0);
+        if (pair >= 0) p[i1] = (int16_t)turn(x0, s[0], x1, c[0]);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const int16_t* x, size_t rows, size_t heads, size_t hd, size_t ldx, const nsrl_rotary& rot,
+                          const int32_t* positions, size_t seq_len, bool backward, int16_t* y, size_t ldy,
+                          cudaStream_t s) {
+  if (rows == 0 || heads == 0) return cudaSuccess;
+  RotArgs a{};
+  a.x = x;
+  a.y = y;
+  a.ldx = (long long)ldx;
+  a.ldy = (long long)ldy;
+  a.rows = (long long)rows;
+  a.turns = reinterpret_cast<const unsigned long long*>(rot.turns);
+  a.positions = positions;
+  a.seq_len = (long long)seq_len;
+  a.heads = (int)heads;
+  a.hd = (int)hd;
+  a.half = (int)(rot.rotary_dim / 2);
+  a.interleaved = rot.interleaved != 0;
+  a.backward = backward;
+  a.amplitude = rot.amplitude;
+  const bool vec = hd % 16 == 0 && a.half % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+  // Rows of a block: about ITEMS items a thread, at least one block an SM
+  // while there are rows for it, and angles that fit the shared memory.
+  const size_t per_row = std::max<size_t>(1, heads * (vec ? hd / 16 : hd - (size_t)a.half));
+  size_t r = std::max<size_t>(1, (size_t)(ITEMS * THREADS) / per_row);
+  r = std::min(r, std::max<size_t>(1, rows / 148));
+  r = std::min(r, std::max<size_t>(1, (size_t)MAX_PAIRS / (size_t)a.half));
+  a.block_rows = (int)r;
+  const size_t blocks = (rows + r - 1) / r;
+  if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+  const double n = (double)rows * (double)heads * (double)hd;
+  ProfScope prof("rotary", s, 3.0 * (double)rows * (double)heads * (double)rot.rotary_dim, 4.0 * n);
+  const cudaError_t e = launch_pdl(vec ? rotary_kernel<true> : rotary_kernel<false>, dim3((unsigned)blocks),
+                                   dim3(THREADS), 8 * r * (size_t)a.half, s, a);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace nsrl
