@@ -28,6 +28,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "common.cuh"
 #include "internal.h"
@@ -49,6 +50,7 @@ struct Q4Shape {
   static constexpr int PAIRS = (G + 1) / 2;              // pairs of groups, 64 dims each
   static constexpr int SHIFT = HD == 16 ? 2 : HD == 64 ? 3 : 4;
   static constexpr int TILE = HD == 16 ? 512 : HD == 64 ? 256 : 128;  // slots of a stage
+  static constexpr int UNIT = HD == 256 ? 16 : 32;  // slots of a warp's step through the keys
   static constexpr int STAGES = HD == 256 ? 3 : 4;
   static constexpr int CODE_BYTES = TILE * HD / 2, SCALE_BYTES = TILE * G * 4;
   static constexpr int STAGE_BYTES = CODE_BYTES + SCALE_BYTES;
@@ -117,7 +119,19 @@ __device__ __forceinline__ void mma_u8u8(int (&c)[4], const uint32_t (&a)[4], co
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-constexpr uint32_t LOW = 0x0F0F0F0Fu;
+__device__ __forceinline__ int add_sat(int x, int y) {
+  int r;
+  asm("add.sat.s32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+
+constexpr uint32_t LOW = 0x0F0F0F0Fu, HIGH = 0xF0F0F0F0u;
+
+// Byte t of the words of a quad's four lanes, in lane order (a 4 x 4 byte transpose).
+__device__ __forceinline__ uint32_t quad_plane(uint32_t x, int t) {
+  x = __byte_perm(x, __shfl_xor_sync(0xffffffffu, x, 2), (t & 2) ? 0x3276 : 0x5410);
+  return __byte_perm(x, __shfl_xor_sync(0xffffffffu, x, 1), (t & 1) ? 0x3715 : 0x6240);
+}
 
 // Code word `t` of every 32-dim group of a slot's row in shared memory.  Rows
 // of 64 and 256 dims are 32 and 128 bytes apart, so lanes of different slots
@@ -258,10 +272,8 @@ __global__ void __launch_bounds__(THREADS) attend_q4_kernel(const AttendArgs a) 
     const uint32_t* codes = reinterpret_cast<const uint32_t*>(dyn + s * S::STAGE_BYTES);
     const uint32_t* scales = reinterpret_cast<const uint32_t*>(dyn + s * S::STAGE_BYTES + S::CODE_BYTES);
     const int left = n - it * S::TILE;
-#pragma unroll
-    for (int u = 0; u < S::TILE / 16; u += WARPS) {
-      const int r = 16 * (u + warp);
-      if (r >= left) break;
+    // 16 slots from r: lanes t even end with slot g's part of group t >> 1, odd ones with slot g + 8's
+    auto dots = [&](int r) -> long long {
       uint32_t w0[S::G], w1[S::G];
       key_words<HD>(codes + (r + g) * S::WORDS, g, t, w0);
       key_words<HD>(codes + (r + g + 8) * S::WORDS, g, t, w1);
@@ -278,16 +290,27 @@ __global__ void __launch_bounds__(THREADS) attend_q4_kernel(const AttendArgs a) 
         v0 += (long long)(alpha * c[0] + beta * c[1]) * (int)(s0 & 0xFFFF) + (long long)qsum[p] * ((int)s0 >> 16);
         v1 += (long long)(alpha * c[2] + beta * c[3]) * (int)(s1 & 0xFFFF) + (long long)qsum[p] * ((int)s1 >> 16);
       }
-      if (S::G == 1 && t >= 2) v0 = v1 = 0;
-      // the quad's four parts: lanes t = 0, 2 end with slot g, lanes t = 1, 3 with slot g + 8
-      const bool odd = t & 1;
-      long long v = odd ? v1 : v0;
-      v += __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
-      v += __shfl_xor_sync(0xffffffffu, v, 2);
-      const int slot = r + g + (odd ? 8 : 0);
-      if (t < 2 && slot < left) {
+      const long long keep = (t & 1) ? v1 : v0;
+      return keep + __shfl_xor_sync(0xffffffffu, (t & 1) ? v0 : v1, 1);
+    };
+#pragma unroll
+    for (int u = 0; u < S::TILE; u += WARPS * S::UNIT) {
+      const int r = u + S::UNIT * warp;
+      if (r >= left) break;
+      int slot = r + g + 8 * (t & 1);
+      bool live = true;
+      long long v = dots(r);
+      if constexpr (S::UNIT == 32) {  // lanes t >= 2 finish the second 16 slots
+        const long long w = dots(r + 16);
+        v = ((t & 2) ? w : v) + __shfl_xor_sync(0xffffffffu, (t & 2) ? v : w, 2);
+        slot += 8 * (t & 2);
+      } else {
+        v += __shfl_xor_sync(0xffffffffu, v, 2);
+        live = t < 2;
+      }
+      if (live && slot < left) {
         const long long lg = v >> S::SHIFT;
-        if (lg != (long long)(int)lg) bad = true;
+        bad = bad || lg != (long long)(int)lg;
         logits[it * S::TILE + slot] = (int)lg;
         mx = max(mx, (int)lg);  // MASKED_LOGIT is INT_MIN: it never raises the maximum
       }
@@ -308,11 +331,14 @@ __global__ void __launch_bounds__(THREADS) attend_q4_kernel(const AttendArgs a) 
 
   // ---------------------------------------------------------------- softmax
   unsigned long long sum = 0;
+#pragma unroll 4
   for (int j = tid; j < n; j += CONSUMERS) {
     const int lg = logits[j];
-    const int w = lg == INT_MIN ? 0 : exp2_neg_q15(lut, (long long)lg - mx);
+    // exp2_neg_q15 of lg - mx <= 0, whose magnitude fits 32 bits
+    const unsigned mag = (unsigned)mx - (unsigned)lg;
+    const int w = lg == INT_MIN || mag >= 15u * 256u ? 0 : (int)lut[mag & 255] >> (mag >> 8);
     logits[j] = w;
-    sum += (unsigned long long)w;
+    sum += (unsigned)w;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -324,18 +350,19 @@ __global__ void __launch_bounds__(THREADS) attend_q4_kernel(const AttendArgs a) 
   alive = exchange(cluster, s_sum, &exchanged[1], sum, part, parts, a.st) && alive;
   sum = 0;
   for (int r = 0; r < parts; ++r) sum += s_sum[r];
-  const long long inv = any ? (long long)recip_sum_q31(sum) : 0;
+  // The slot at the maximum has weight 32767, so sum >= 32767, inv <= 65793 and
+  // w inv + 2^15 < 2^32: sat_i16(rhu64(w * inv, 16)) in 32 bits.
+  const unsigned inv = any ? recip_sum_q31(sum) : 0u;
   const int padded = (n + SHARE_UNIT - 1) / SHARE_UNIT * SHARE_UNIT;
+  int32_t* const scores = a.c.scores ? a.c.scores + slot0 : nullptr;
+#pragma unroll 4
   for (int j = tid; j < padded; j += CONSUMERS) {
     if (j >= n) {
       logits[j] = 0;  // slots of the last value MMA past the share weigh nothing
-      continue;
-    }
-    const int p = (int)sat_i16(rhu64((long long)logits[j] * inv, 16));
-    logits[j] = p;
-    if (a.c.scores) {
-      const long long sc = (long long)a.c.scores[slot0 + j] + p;
-      a.c.scores[slot0 + j] = (int32_t)min(sc, 2147483647ll);
+    } else {
+      const int p = (int)min(((unsigned)logits[j] * inv + 32768u) >> 16, 32767u);
+      logits[j] = p;
+      if (scores) scores[j] = add_sat(scores[j], p);
     }
   }
   consumers_sync();
@@ -344,16 +371,21 @@ __global__ void __launch_bounds__(THREADS) attend_q4_kernel(const AttendArgs a) 
   // A warp's unit is 32 slots of one pair of groups (64 dims).  Lane (g, t)
   // reads code word g of the pair for slots 4 j + t; byte i of it holds dims
   // 2 i and 2 i + 1, rows g and g + 8 of MMA i (16 dims a head: byte g, MMA 0).
+  // High halves are left in place (16 times the code: rows g + 8 shift down at
+  // the end).  The weights p scale are formed once per slot and group, on lane
+  // 4 (slot & 3 | slot >> 4 & 1 << 2) + (slot >> 2 & 3), and their byte planes
+  // handed to the lanes of their column.
   constexpr int MMAS = HD == 16 ? 1 : 4;
   const int pair = warp % S::PAIRS;
-  const int vgroup = S::G == 1 ? 0 : 2 * pair + (g >> 2);
   int acc[MMAS][4];
 #pragma unroll
   for (int i = 0; i < MMAS; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = 0;
-  long long zacc = 0;
-  const uint32_t plane2 = (uint32_t)(g & 3) | ((uint32_t)((g & 3) + 4) << 4);  // that byte of two words
+  long long zero_part[2] = {0, 0};  // sum of p zero over this lane's slots, per group of the pair
+  const int own = 4 * t + (g & 3) + 16 * (g >> 2);  // the slot whose weights this lane forms
+  const int from = 4 * t + (g & 3);                 // the lane with plane g & 3 of slots 4 i + t
+  const uint32_t byte2 = (uint32_t)(g & 3) | ((uint32_t)((g & 3) + 4) << 4);  // byte g & 3 of two words
   for (int it = tiles; it < 2 * tiles && alive; ++it) {
     const int s = it % S::STAGES;
     alive = mbar_wait(&full[s], (it / S::STAGES) & 1, a.st);
@@ -364,27 +396,36 @@ __global__ void __launch_bounds__(THREADS) attend_q4_kernel(const AttendArgs a) 
     for (int u = 0; u < S::TILE / 32; u += WARPS / S::PAIRS) {
       const int r = 32 * (u + warp / S::PAIRS);
       if (r >= left) break;
-      uint32_t w[8], pw[8];
+      uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int slot = r + 4 * j + t;
-        w[j] = codes[slot * S::WORDS + (HD == 16 ? g >> 2 : 8 * pair + g)];
-        const int p = logits[at + slot];
-        const uint32_t sw = scales[slot * S::G + vgroup];
-        pw[j] = (uint32_t)p * (sw & 0xFFFF);
-        zacc += (long long)p * ((int)sw >> 16);
-      }
+      for (int j = 0; j < 8; ++j) w[j] = codes[(r + 4 * j + t) * S::WORDS + (HD == 16 ? g >> 2 : 8 * pair + g)];
+      const int p = logits[at + r + own];
       uint32_t bf[2];
+      if constexpr (HD == 16) {
+        const uint32_t sw = scales[r + own];
+        zero_part[0] += (long long)p * ((int)sw >> 16);
+        const uint32_t plane = quad_plane((uint32_t)p * (sw & 0xFFFF), t);
+        bf[0] = __shfl_sync(0xffffffffu, plane, from);
+        bf[1] = __shfl_sync(0xffffffffu, plane, from + 16);
+      } else {
+        const uint2 sw = *reinterpret_cast<const uint2*>(scales + (r + own) * S::G + 2 * pair);
+        zero_part[0] += (long long)p * ((int)sw.x >> 16);
+        zero_part[1] += (long long)p * ((int)sw.y >> 16);
+        const uint32_t plane0 = quad_plane((uint32_t)p * (sw.x & 0xFFFF), t);
+        const uint32_t plane1 = quad_plane((uint32_t)p * (sw.y & 0xFFFF), t);
 #pragma unroll
-      for (int o = 0; o < 2; ++o)
-        bf[o] = __byte_perm(__byte_perm(pw[4 * o], pw[4 * o + 1], plane2), __byte_perm(pw[4 * o + 2], pw[4 * o + 3], plane2),
-                            0x5410);
+        for (int o = 0; o < 2; ++o) {
+          const uint32_t x = __shfl_sync(0xffffffffu, plane0, from + 16 * o);
+          const uint32_t y = __shfl_sync(0xffffffffu, plane1, from + 16 * o);
+          bf[o] = (g >> 2) ? y : x;
+        }
+      }
       uint32_t by[2][MMAS];  // byte i of four slots' words
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
-        const uint32_t *x = w + 4 * o;
+        const uint32_t* x = w + 4 * o;
         if constexpr (HD == 16) {
-          by[o][0] = __byte_perm(__byte_perm(x[0], x[1], plane2), __byte_perm(x[2], x[3], plane2), 0x5410);
+          by[o][0] = __byte_perm(__byte_perm(x[0], x[1], byte2), __byte_perm(x[2], x[3], byte2), 0x5410);
         } else {
           const uint32_t lo01 = __byte_perm(x[0], x[1], 0x5140), hi01 = __byte_perm(x[0], x[1], 0x7362);
           const uint32_t lo23 = __byte_perm(x[2], x[3], 0x5140), hi23 = __byte_perm(x[2], x[3], 0x7362);
@@ -396,7 +437,7 @@ __global__ void __launch_bounds__(THREADS) attend_q4_kernel(const AttendArgs a) 
       }
 #pragma unroll
       for (int i = 0; i < MMAS; ++i) {
-        const uint32_t frag[4] = {by[0][i] & LOW, (by[0][i] >> 4) & LOW, by[1][i] & LOW, (by[1][i] >> 4) & LOW};
+        const uint32_t frag[4] = {by[0][i] & LOW, by[0][i] & HIGH, by[1][i] & LOW, by[1][i] & HIGH};
         mma_u8u8(acc[i], frag, bf);
       }
     }
@@ -404,18 +445,24 @@ __global__ void __launch_bounds__(THREADS) attend_q4_kernel(const AttendArgs a) 
     if (lane == 0) mbar_arrive(&empty[s]);
   }
   // Columns 2 t and 2 t + 1 are planes 2 (t & 1) and 2 (t & 1) + 1 of the pair's
-  // group t >> 1; the lane's dims are of group g >> 2 of the pair.
-  zacc += __shfl_xor_sync(0xffffffffu, zacc, 1);
-  zacc += __shfl_xor_sync(0xffffffffu, zacc, 2);
+  // group t >> 1; the lane's dims are of group g >> 2 of the pair.  s32 is enough:
+  // 240 * 255 a slot over at most 16,384 slots a warp.
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    zero_part[0] += __shfl_xor_sync(0xffffffffu, zero_part[0], o);
+    if (HD != 16) zero_part[1] += __shfl_xor_sync(0xffffffffu, zero_part[1], o);
+  }
+  const long long zeros = HD != 16 && (g >> 2) ? zero_part[1] : zero_part[0];
   const bool mine = (t & 1) == 0 && (HD == 16 ? t == 0 : (t >> 1) == (g >> 2));
 #pragma unroll
   for (int i = 0; i < MMAS; ++i)
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
-      long long v = ((long long)acc[i][2 * o] + ((long long)acc[i][2 * o + 1] << 8)) << (16 * (t & 1));
+      const int lo = acc[i][2 * o] >> (4 * o), hi = acc[i][2 * o + 1] >> (4 * o);
+      long long v = ((long long)lo + ((long long)hi << 8)) << (16 * (t & 1));
       v += __shfl_xor_sync(0xffffffffu, v, 1);
       const int dim = HD == 16 ? 2 * g + o : 64 * pair + 8 * g + 2 * i + o;
-      if (mine) atomicAdd(&s_ctx[dim], (unsigned long long)(v + zacc));
+      if (mine) atomicAdd(&s_ctx[dim], (unsigned long long)(v + zeros));
     }
   cluster.sync();
   if (part == 0 && tid < HD) {
@@ -461,6 +508,7 @@ cudaError_t launch_attend_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache& 
   while (parts < MAX_CLUSTER &&
          ((c.capacity + parts - 1) / parts > MAX_SHARE || (bh * parts < 148 && c.capacity / parts >= 512)))
     parts *= 2;
+  if (getenv("Q4PARTS")) parts = atoi(getenv("Q4PARTS"));
   const size_t share = ((c.capacity + parts - 1) / parts + SHARE_UNIT - 1) / SHARE_UNIT * SHARE_UNIT;
   const double slots = (double)bh * (double)c.capacity;
   ProfScope prof("attention_decode_q4", s, 4.0 * slots * (double)c.head_dim,
