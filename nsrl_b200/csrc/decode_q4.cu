@@ -22,10 +22,12 @@
 //           groups, one column each.  An MMA takes 32 cycles of its quarter SM,
 //           one cycle a slot in all; for the keys, whose products need no
 //           transpose, dp4a costs fewer instructions.
-// Everything is exact in s32 until it is combined in 64 bits.  One warp
-// streams tiles of codes and scales (K, then V) through a ring of bulk copies,
-// so value tiles arrive while the softmax runs; groups of consumer warps take
-// the tiles in turn, so that one group's latencies hide behind the others'.
+// Everything is exact in s32 until it is combined in 64 bits.  Two warps
+// stream tiles of codes and scales (K, then V) through a ring of bulk copies,
+// so value tiles arrive while the softmax runs (waiting for a stage and
+// refilling it takes a warp about 375 cycles whatever the size, more than a
+// tile's share of the memory's time: hence two).  Teams of consumer warps take
+// the tiles in turn, so that one team's latencies hide behind the others'.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -38,7 +40,8 @@ namespace cg = cooperative_groups;
 namespace nsrl {
 namespace {
 
-constexpr int WARPS = 16, CONSUMERS = 32 * WARPS, THREADS = CONSUMERS + 32;
+constexpr int WARPS = 16, COPIERS = 2;
+constexpr int CONSUMERS = 32 * WARPS, THREADS = CONSUMERS + 32 * COPIERS;
 constexpr int MAX_CLUSTER = 16;
 constexpr int SHARE_UNIT = 32;       // slots of a value MMA
 constexpr size_t MAX_SHARE = 32768;  // logits of a CTA: 128 KB
@@ -147,9 +150,10 @@ __device__ __forceinline__ uint32_t quad_plane(uint32_t x, int t) {
 }
 
 // Weight of a logit (exp2_neg_q15 of lg - mx <= 0, whose magnitude fits 32 bits).
+// From 15 * 256 on it is 0: so is MASKED_LOGIT's, INT_MIN, unless mx is that low.
 __device__ __forceinline__ unsigned weight(const int16_t* lut, int lg, int mx) {
-  const unsigned mag = (unsigned)mx - (unsigned)lg;
-  return lg == INT_MIN || mag >= 15u * 256u ? 0u : (unsigned)lut[mag & 255] >> (mag >> 8);
+  const unsigned mag = min((unsigned)mx - (unsigned)lg, 15u * 256u);
+  return (unsigned)lut[mag & 255] >> (mag >> 8);
 }
 
 template <int HD>
@@ -164,12 +168,13 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
   // per group and code word {h of the even dims, h of the odd dims, l even, l odd}; then the group's sum of q
   __shared__ __align__(16) uint32_t s_q[S::G * S::Q_STRIDE];
   __shared__ int s_max[MAX_CLUSTER], s_redi[WARPS];
-  __shared__ unsigned long long s_sum[MAX_CLUSTER], s_red[WARPS];
+  __shared__ unsigned s_red[WARPS];
+  __shared__ unsigned long long s_sum[MAX_CLUSTER];
   __shared__ long long s_part[WARPS / S::PAIRS][HD], s_ctx[HD];
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == CONSUMERS) {  // the copying thread, which goes on without a barrier
+  if (tid == CONSUMERS) {  // the copying warps do not wait for the others
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], S::TEAM);
@@ -203,15 +208,18 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
   const size_t slot0 = (size_t)bh * a.c.capacity + (size_t)first;
   const int tiles = (n + S::TILE - 1) / S::TILE;
 
-  if (warp == WARPS) {
-    // ---------------------------------------------------------------- producer
-    if (parts > 1)
-      cluster.sync();
-    else
-      asm volatile("bar.arrive 2, %0;" ::"n"(THREADS) : "memory");  // the barriers are ready
+  if (warp >= WARPS) {
+    // ---------------------------------------------------------------- copies
+    if (parts > 1) {
+      cluster.sync();  // every CTA's barriers are ready
+    } else {
+      asm volatile("bar.sync 3, %0;" ::"n"(32 * COPIERS) : "memory");
+      asm volatile("bar.arrive 2, %0;" ::"n"(THREADS) : "memory");
+    }
     if (lane == 0) {
+      static_assert(S::STAGES % COPIERS == 0);
       int issued = 0;
-      for (int it = 0; it < 2 * tiles; ++it) {
+      for (int it = warp - WARPS; it < 2 * tiles; it += COPIERS) {
         const int s = it % S::STAGES;
         if (it >= S::STAGES && !mbar_wait(&empty[s], ((it / S::STAGES) - 1) & 1, a.st)) break;
         const bool value = it >= tiles;
@@ -225,7 +233,8 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
                   &full[s]);
         issued = it + 1;
       }
-      for (int it = (issued > S::STAGES ? issued - S::STAGES : 0); it < issued; ++it)
+      // the copies in flight land before the CTA may leave: this warp's last ones, one a stage
+      for (int it = issued - 1; it >= 0 && it > issued - 1 - S::STAGES; it -= COPIERS)
         mbar_wait(&full[it % S::STAGES], (it / S::STAGES) & 1, a.st);
     }
     __syncwarp();
@@ -362,22 +371,26 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
   if (!any && tid == 0 && part == 0) nsrl_flag(a.st, NSRL_FLAG_ALL_MASKED);
 
   // ---------------------------------------------------------------- softmax
-  // Weights replace the logits; zeros fill the last value MMA past the share.
-  const int padded = (n + SHARE_UNIT - 1) / SHARE_UNIT * SHARE_UNIT;
-  unsigned long long sum = 0;
+  // Only the sum: the value pass weighs each slot again.  A CTA's sum is at most
+  // 2^15 * MAX_SHARE = 2^30.
+  unsigned part_sum = 0;
+  const bool low = mx < INT_MIN + 15 * 256;  // MASKED_LOGIT would gather weight
+  const int none = (int)((unsigned)mx - 15u * 256u);
 #pragma unroll 2
-  for (int j = 4 * tid; j < padded; j += 4 * CONSUMERS) {
-    const int4 lg = *reinterpret_cast<const int4*>(logits + j);
-    const int4 w = make_int4(j < n ? (int)weight(lut, lg.x, mx) : 0, j + 1 < n ? (int)weight(lut, lg.y, mx) : 0,
-                             j + 2 < n ? (int)weight(lut, lg.z, mx) : 0, j + 3 < n ? (int)weight(lut, lg.w, mx) : 0);
-    *reinterpret_cast<int4*>(logits + j) = w;
-    sum += (unsigned)(w.x + w.y + w.z + w.w);
+  for (int j = 4 * tid; j < n; j += 4 * CONSUMERS) {
+    int4 lg = *reinterpret_cast<const int4*>(logits + j);
+    if (j + 3 >= n || low) {
+      if (lg.x == INT_MIN) lg.x = none;
+      if (lg.y == INT_MIN || j + 1 >= n) lg.y = none;
+      if (lg.z == INT_MIN || j + 2 >= n) lg.z = none;
+      if (lg.w == INT_MIN || j + 3 >= n) lg.w = none;
+    }
+    part_sum += weight(lut, lg.x, mx) + weight(lut, lg.y, mx) + weight(lut, lg.z, mx) + weight(lut, lg.w, mx);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_red[warp] = sum;
+  part_sum = __reduce_add_sync(0xffffffffu, part_sum);
+  if (lane == 0) s_red[warp] = part_sum;
   consumers_sync();
-  sum = 0;
+  unsigned long long sum = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) sum += s_red[w];
   if (parts > 1) {
@@ -398,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
   // reads code word g of the pair for slots 4 j + t; byte i of it holds dims
   // 2 i and 2 i + 1, rows g and g + 8 of MMA i (16 dims a head: byte g, MMA 0).
   // High halves are left in place (16 times the code: rows g + 8 shift down at
-  // the end).  Slot `own` is this lane's to weigh (p, its score, p scale); the
+  // the end).  Slot `own` is this lane's to weigh (p, its score, p scale: 0 past the share); the
   // byte planes of p scale then go to the lanes of their column.
   constexpr int MMAS = HD == 16 ? 1 : 4;
   const int g = lane >> 2, t = lane & 3;
@@ -430,7 +443,6 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
     alive = mbar_wait(&full[s], (it / S::STAGES) & 1, a.st);
     const uint32_t* codes = reinterpret_cast<const uint32_t*>(dyn + s * S::STAGE_BYTES);
     const uint32_t* scales = reinterpret_cast<const uint32_t*>(dyn + s * S::STAGE_BYTES + S::CODE_BYTES);
-    // A slot past the share has a weight of 0 (logits are padded to 32 slots; beyond, the unit is left out).
     uint32_t w[UNITS][8];
     uint2 sw[UNITS];
     auto load = [&](int k) {
@@ -453,7 +465,9 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
       const int r = 32 * (k * STEP + mate / S::PAIRS);
       if (r >= left) break;
       if constexpr (HD == 256) load(k);
-      const int p = (int)min(((unsigned)logits[at + r + own] * inv + 32768u) >> 16, 32767u);
+      const int lg = logits[at + r + own];
+      const bool masked = r + own >= left || lg == INT_MIN;
+      const int p = masked ? 0 : (int)min((weight(lut, lg, mx) * inv + 32768u) >> 16, 32767u);
       if (scores && r + own < left) scores[at + r + own] = add_sat(old[k], p);
       uint32_t bf[2];
       zero_part[0] += (long long)p * ((int)sw[k].x >> 16);
