@@ -141,6 +141,14 @@ __device__ __forceinline__ int add_sat(int x, int y) {
   return r;
 }
 
+// Four 8 x 8 matrices of 16-bit elements, transposed; lane l gives the 16-byte row l & 7 of matrix l >> 3.
+__device__ __forceinline__ void load_matrices(uint32_t row, uint32_t* w) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "r"(row)
+               : "memory");
+}
+
 constexpr uint32_t LOW = 0x0F0F0F0Fu, HIGH = 0xF0F0F0F0u;
 
 // Byte t of the words of a quad's four lanes, in lane order (a 4 x 4 byte transpose).
@@ -165,7 +173,7 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
   __shared__ uint64_t exchanged[2];  // the cluster's maxima and sums are here
   __shared__ int16_t lut[256];
   __shared__ uint32_t recip[128];
-  // per group and code word {h of the even dims, h of the odd dims, l even, l odd}; then the group's sum of q
+  // per group and code word {h of the even dims, h of the odd dims, l even, l odd}; then 16 times the group's sum of q
   __shared__ __align__(16) uint32_t s_q[S::G * S::Q_STRIDE];
   __shared__ int s_max[MAX_CLUSTER], s_redi[WARPS];
   __shared__ unsigned s_red[WARPS];
@@ -259,7 +267,7 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
     for (int o = 1; o < S::GW; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
     uint32_t* group = s_q + (tid / S::GW) * S::Q_STRIDE;
     *reinterpret_cast<uint4*>(group + 4 * (tid % S::GW)) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (tid % S::GW == 0) group[4 * S::GW] = (uint32_t)sum;
+    if (tid % S::GW == 0) group[4 * S::GW] = (uint32_t)(16 * sum);
   }
   if (parts > 1)
     cluster.sync();
@@ -331,7 +339,7 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
           w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
           sw = scales[slot * S::G + c];
         }
-        // even dims; and odd dims in the high half bytes, 16 times over
+        // odd dims stay in the high half bytes, 16 times over: the even dims' sums catch up
         int he = 0, ho = 0, le = 0, lo = 0;
 #pragma unroll
         for (int k = 0; k < S::GW; ++k) {
@@ -341,12 +349,12 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
           le = dp4a_uu(w[k] & LOW, q.z, le);
           lo = dp4a_uu(w[k] & HIGH, q.w, lo);
         }
-        const int dot = he * 256 + le + ((ho * 256 + lo) >> 4);
+        const int dot = (he * 256 + le) * 16 + (ho * 256 + lo);  // 16 sum q code, below 2^28
         const int qsum = HELD ? qs[i] : (int)s_q[c * S::Q_STRIDE + 4 * S::GW];
         v += (long long)dot * (int)(sw & 0xFFFF) + (long long)qsum * ((int)sw >> 16);
       }
       if (slot < left) {
-        const long long lg = v >> S::SHIFT;
+        const long long lg = v >> (S::SHIFT + 4);
         bad = bad || lg != (long long)(int)lg;
         logits[it * S::TILE + slot] = (int)lg;
         mx = max(mx, (int)lg);  // MASKED_LOGIT is INT_MIN: it never raises the maximum
@@ -407,11 +415,13 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
   }
 
   // ------------------------------------------------------------------ values
-  // A warp's unit is 32 slots of one pair of groups (64 dims).  Lane (g, t)
-  // reads code word g of the pair for slots 4 j + t; byte i of it holds dims
-  // 2 i and 2 i + 1, rows g and g + 8 of MMA i (16 dims a head: byte g, MMA 0).
-  // High halves are left in place (16 times the code: rows g + 8 shift down at
-  // the end).  Slot `own` is this lane's to weigh (p, its score, p scale: 0 past the share); the
+  // A warp's unit is 32 slots of one pair of groups (64 dims).  Transposing
+  // matrix loads give lane (g, t) bytes 2 g and 2 g + 1 of a group's row for
+  // slots 8 m + 2 t and 8 m + 2 t + 1; two loads and a PRMT make one byte of four
+  // slots.  16 dims a head (8-byte rows): byte g of slots 4 j + t from words.  A
+  // byte holds an even and an odd dim: row g of its MMA takes the byte as it is
+  // (even + 16 odd), row g + 8 its high half (16 odd), and they part at the
+  // end.  Slot `own` is this lane's to weigh (p, its score, p scale: 0 past the share); the
   // byte planes of p scale then go to the lanes of their column.
   constexpr int MMAS = HD == 16 ? 1 : 4;
   const int g = lane >> 2, t = lane & 3;
@@ -422,8 +432,9 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = 0;
   long long zero_part[2] = {0, 0};  // sum of p zero over this lane's slots, per group of the pair
-  const int own = 4 * t + (g & 3) + 16 * (g >> 2);
-  const int from = 4 * t + (g & 3);  // the lane with plane g & 3 of slots 4 i + t; 16 further, of slots 16 + 4 i + t
+  // The quad's slots are those of k = 4 (g & 3) + 16 (g >> 2) and the three after it.
+  const int own = 16 * (g >> 2) + (HD == 16 ? 4 * t + (g & 3) : 8 * (t >> 1) + 2 * (g & 3) + (t & 1));
+  const int from = 4 * t + (g & 3);  // the lane with plane g & 3 of the slots of k = 4 t; 16 further, of 16 + 4 t
   const uint32_t byte2 = (uint32_t)(g & 3) | ((uint32_t)((g & 3) + 4) << 4);  // byte g & 3 of two words
   int32_t* const scores = a.c.scores && pair == 0 ? a.c.scores + slot0 : nullptr;
   // A stage stays with one team for both passes, so that no wait skips a phase.
@@ -447,12 +458,17 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
     uint2 sw[UNITS];
     auto load = [&](int k) {
       const int r = 32 * (k * STEP + mate / S::PAIRS);
+      if constexpr (HD == 16) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[k][j] = codes[(r + 4 * j + t) * S::WORDS + (HD == 16 ? g >> 2 : 8 * pair + g)];
-      if constexpr (HD == 16)
+        for (int j = 0; j < 8; ++j) w[k][j] = codes[(r + 4 * j + t) * S::WORDS + (g >> 2)];
         sw[k] = make_uint2(scales[r + own], 0);
-      else
+      } else {
+        // lane l points at row r + l; w[k][4 e + m] is group e of slots 8 m ..
+        const uint32_t row = smem_u32(codes + (r + lane) * S::WORDS + 8 * pair);
+        load_matrices(row, w[k]);
+        load_matrices(row + 16, w[k] + 4);
         sw[k] = *reinterpret_cast<const uint2*>(scales + (r + own) * S::G + 2 * pair);
+      }
     };
     if constexpr (HD != 256) {
 #pragma unroll
@@ -485,24 +501,18 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
           bf[o] = (g >> 2) ? y : x;
         }
       }
-      uint32_t by[2][MMAS];  // byte i of four slots' words
-#pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        const uint32_t* x = w[k] + 4 * o;
-        if constexpr (HD == 16) {
-          by[o][0] = __byte_perm(__byte_perm(x[0], x[1], byte2), __byte_perm(x[2], x[3], byte2), 0x5410);
-        } else {
-          const uint32_t lo01 = __byte_perm(x[0], x[1], 0x5140), hi01 = __byte_perm(x[0], x[1], 0x7362);
-          const uint32_t lo23 = __byte_perm(x[2], x[3], 0x5140), hi23 = __byte_perm(x[2], x[3], 0x7362);
-          by[o][0] = __byte_perm(lo01, lo23, 0x5410);
-          by[o][1] = __byte_perm(lo01, lo23, 0x7632);
-          by[o][2] = __byte_perm(hi01, hi23, 0x5410);
-          by[o][3] = __byte_perm(hi01, hi23, 0x7632);
-        }
-      }
 #pragma unroll
       for (int i = 0; i < MMAS; ++i) {
-        const uint32_t frag[4] = {by[0][i] & LOW, by[0][i] & HIGH, by[1][i] & LOW, by[1][i] & HIGH};
+        uint32_t x, y;  // the byte of k = 4 t .. and of k = 16 + 4 t ..
+        if constexpr (HD == 16) {
+          x = __byte_perm(__byte_perm(w[k][0], w[k][1], byte2), __byte_perm(w[k][2], w[k][3], byte2), 0x5410);
+          y = __byte_perm(__byte_perm(w[k][4], w[k][5], byte2), __byte_perm(w[k][6], w[k][7], byte2), 0x5410);
+        } else {  // MMA i: byte i & 1 of group i >> 1
+          const uint32_t* m = w[k] + 4 * (i >> 1);
+          x = __byte_perm(m[0], m[1], (i & 1) ? 0x7531 : 0x6420);
+          y = __byte_perm(m[2], m[3], (i & 1) ? 0x7531 : 0x6420);
+        }
+        const uint32_t frag[4] = {x, x & HIGH, y, y & HIGH};
         mma_u8u8(acc[i], frag, bf);
       }
     }
@@ -511,25 +521,22 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
       if (lane == 0) mbar_arrive(&empty[s]);
     }
   }
-  // Columns 2 t and 2 t + 1 are planes 2 (t & 1) and 2 (t & 1) + 1 of the pair's
-  // group t >> 1; the lane's dims are of group g >> 2 of the pair.  s32 is enough:
-  // 240 * 255 a slot over at most 8,192 slots a warp.
+  // Columns 2 t and 2 t + 1 are planes 2 (t & 1) and 2 (t & 1) + 1 of group t >> 1
+  // of the pair.  s32 is enough: 255 * 255 a slot over at most 8,192 slots a warp.
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     zero_part[0] += __shfl_xor_sync(0xffffffffu, zero_part[0], o);
     if (HD != 16) zero_part[1] += __shfl_xor_sync(0xffffffffu, zero_part[1], o);
   }
-  const long long zeros = HD != 16 && (g >> 2) ? zero_part[1] : zero_part[0];
-  const bool mine = (t & 1) == 0 && (HD == 16 ? t == 0 : (t >> 1) == (g >> 2));
 #pragma unroll
   for (int i = 0; i < MMAS; ++i)
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
-      const int lo = acc[i][2 * o] >> (4 * o), hi = acc[i][2 * o + 1] >> (4 * o);
-      long long v = ((long long)lo + ((long long)hi << 8)) << (16 * (t & 1));
+      const int p0 = o ? acc[i][2] >> 4 : acc[i][0] - acc[i][2], p1 = o ? acc[i][3] >> 4 : acc[i][1] - acc[i][3];
+      long long v = ((long long)p0 + ((long long)p1 << 8)) << (16 * (t & 1));
       v += __shfl_xor_sync(0xffffffffu, v, 1);
-      const int dim = HD == 16 ? 2 * g + o : 64 * pair + 8 * g + 2 * i + o;
-      if (mine) s_part[warp / S::PAIRS][dim] = v + zeros;
+      const int dim = HD == 16 ? 2 * g + o : 64 * pair + 32 * (i >> 1) + 4 * g + 2 * (i & 1) + o;
+      if (t == 2 * (i >> 1)) s_part[warp / S::PAIRS][dim] = v + zero_part[i >> 1];
     }
   consumers_sync();
   long long total = 0;
