@@ -574,7 +574,7 @@ cudaError_t launch_attend(const AttendArgs& a, int parts, size_t share, cudaStre
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = parts > 1 ? 2 : 1;  // a cluster of one would be packed two to an SM while others idle
   return cudaLaunchKernelEx(&cfg, attend_q4_kernel<HD>, a);
 }
 
