@@ -917,6 +917,7 @@ nsrl_status nsrl_q4_cache_append(const nsrl_q4_cache* cache, const int16_t* k, c
   if (r != NSRL_OK) return r;
   if (ld < cache->heads * cache->head_dim) return shape_fail("append: rows shorter than heads * head_dim");
   if (tokens > cache->capacity) return shape_fail("append: more tokens than the capacity");
+  if (cache->batch * cache->heads * tokens > 0xffffff00u) return shape_fail("append: 2^32 slots or more");
   if (cache->batch == 0 || tokens == 0) return NSRL_OK;
   if (!k || !v || !starts || !status) return shape_fail("NULL argument");
   NSRL_TRY(launch_q4_append(*cache, k, v, ld, tokens, starts, counts, positions, status, (cudaStream_t)stream),
@@ -929,6 +930,7 @@ nsrl_status nsrl_q4_cache_read(const nsrl_q4_cache* cache, const int32_t* starts
   const nsrl_status r = check_q4(cache);
   if (r != NSRL_OK) return r;
   if (tokens > cache->capacity) return shape_fail("read: more tokens than the capacity");
+  if (cache->batch * cache->heads * tokens > 0xffffff00u) return shape_fail("read: 2^32 slots or more");
   if (cache->batch == 0 || tokens == 0) return NSRL_OK;
   if (!k || !v || !status) return shape_fail("NULL argument");
   if (!aligned(k, 16) || !aligned(v, 16)) return shape_fail("read: k and v must be 16-byte aligned");

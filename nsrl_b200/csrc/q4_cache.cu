@@ -23,6 +23,7 @@ struct AppendArgs {
   const int16_t* v;
   long long ld;
   long long tokens;
+  unsigned rows;  // batch * heads * tokens
   const int32_t* starts;
   const int32_t* counts;
   const int32_t* positions;
@@ -76,22 +77,19 @@ __global__ void __launch_bounds__(THREADS) q4_append_kernel(const AppendArgs a, 
   constexpr int G = HD < 32 ? 1 : HD / 32;
   griddep_wait();
   griddep_launch();
-  const long long total = (long long)a.c.batch * a.c.heads * a.tokens * LPR;
-  const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
-  const bool inside = i < total;  // every lane of a warp takes part in the shuffles
-  const int sub = (int)(i % LPR);
-  const long long row = i / LPR;
-  const long long bh = inside ? row / a.tokens : 0;
-  const long long t = row - bh * a.tokens;
-  const int h = (int)(bh % (long long)a.c.heads);
-  const long long b = bh / (long long)a.c.heads;
+  const int sub = threadIdx.x % LPR;
+  const unsigned row = blockIdx.x * (THREADS / LPR) + threadIdx.x / LPR;
+  const bool inside = row < a.rows;  // every lane of a warp takes part in the shuffles
+  const unsigned tokens = (unsigned)a.tokens, heads = (unsigned)a.c.heads;
+  const unsigned bh = inside ? row / tokens : 0, t = inside ? row - bh * tokens : 0;
+  const unsigned b = bh / heads, h = bh - b * heads;
   const long long start = a.starts[b], count = a.counts ? (long long)a.counts[b] : a.tokens;
   const bool fits = start >= 0 && count >= 0 && count <= a.tokens && start + count <= (long long)a.c.capacity;
   if (inside && !fits && t == 0 && sub == 0 && h == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
-  const bool live = inside && fits && t < count;
+  const bool live = inside && fits && (long long)t < count;
   uint4 uk = make_uint4(0, 0, 0, 0), uv = uk;
   if (live) {
-    const long long off = (b * a.tokens + t) * a.ld + (long long)h * HD + 8 * sub;
+    const long long off = ((long long)b * a.tokens + t) * a.ld + (long long)h * HD + 8 * sub;
     uk = load8(a.k + off, vec);
     uv = load8(a.v + off, vec);
   }
@@ -115,6 +113,7 @@ struct ReadArgs {
   nsrl_q4_cache c;
   const int32_t* starts;
   long long tokens;
+  unsigned rows;
   int16_t* k;
   int16_t* v;
   nsrl_device_status* st;
@@ -136,13 +135,12 @@ __global__ void __launch_bounds__(THREADS) q4_read_kernel(const ReadArgs a) {
   constexpr int G = HD < 32 ? 1 : HD / 32;
   griddep_wait();
   griddep_launch();
-  const long long total = (long long)a.c.batch * a.c.heads * a.tokens * LPR;
-  const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
-  if (i >= total) return;
-  const int sub = (int)(i % LPR);
-  const long long row = i / LPR;
-  const long long bh = row / a.tokens, t = row - bh * a.tokens;
-  const long long b = bh / (long long)a.c.heads;
+  const int sub = threadIdx.x % LPR;
+  const unsigned row = blockIdx.x * (THREADS / LPR) + threadIdx.x / LPR;
+  if (row >= a.rows) return;
+  const unsigned tokens = (unsigned)a.tokens;
+  const unsigned bh = row / tokens, t = row - bh * tokens, b = bh / (unsigned)a.c.heads;
+  const size_t i = (size_t)row * LPR + sub;
   const long long start = a.starts ? (long long)a.starts[b] : 0;
   if (start < 0 || start + a.tokens > (long long)a.c.capacity) {
     if (t == 0 && sub == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
@@ -158,12 +156,16 @@ __global__ void __launch_bounds__(THREADS) q4_read_kernel(const ReadArgs a) {
 
 // ------------------------------------------------------------- eviction ----
 // Two launches.  q4_select_kernel (one CTA per (sequence, head)) finds the
-// keep-th largest key by radix selection, 8 bits a pass, where key =
-// 2^31 for a protected slot, else max(score, 0); marks the kept slots (ties to
-// the lower slot) in a shared-memory bitmap; lists the holes below `keep` and
-// the kept slots at or past it, both in ascending order and equally many.
+// keep-th largest key by radix selection, 8 bits a pass from the highest bit in
+// use and no further than the bin that is kept whole, where key = 2^31 for a
+// protected slot, else max(score, 0); marks the kept slots (ties to the lower
+// slot) in a shared-memory bitmap; lists the holes below `keep` and the kept
+// slots at or past it, both in ascending order and equally many.
 // q4_move_kernel copies the m-th listed slot into the m-th hole.  Sources lie
 // at or past `keep` and destinations below it, so the moves need no order.
+constexpr unsigned SAFE = 0x80000000u;  // key of a protected slot, above every score
+constexpr unsigned NONE = 0xFFFFFFFFu;  // no slot
+
 struct EvictArgs {
   nsrl_q4_cache c;
   const int32_t* lens;
@@ -177,19 +179,25 @@ struct EvictArgs {
   nsrl_device_status* st;
 };
 
-constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32;
-
+// The first keys of a thread's span stay in registers (HELD of them, chosen from
+// the capacity); a longer span's others are read again in each pass.  Bound by
+// memory: 8 bytes a slot in, 8 a kept slot out.
+template <int SEL_THREADS, int HELD>
 __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs a) {
-  extern __shared__ uint32_t bitmap[];  // kept slots, [capacity / 32 + 1]
+  constexpr int SEL_WARPS = SEL_THREADS / 32;
+  extern __shared__ uint32_t bitmap[];  // kept slots, 32 a word
   __shared__ int hist[256];
   __shared__ int warp_a[SEL_WARPS], warp_b[SEL_WARPS];
-  __shared__ unsigned s_prefix;
-  __shared__ int s_want;
+  __shared__ unsigned s_prefix, s_top;
+  __shared__ int s_want, s_safe;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    s_top = 0;
+    s_safe = 0;
+  }
   griddep_wait();
   griddep_launch();
-  const long long bh = blockIdx.x;
-  const long long b = bh / (long long)a.c.heads;
+  const unsigned bh = blockIdx.x, b = bh / (unsigned)a.c.heads;
   const int keep = (int)a.keep;
   const int n = a.lens[b];
   if (n < 0 || n > (int)a.c.capacity) {
@@ -199,15 +207,11 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
     }
     return;
   }
-  const int32_t* scores = a.c.scores + bh * (long long)a.c.capacity;
-  const int32_t* positions = a.c.positions + bh * (long long)a.c.capacity;
-  int32_t* scores_out = a.scores_out + bh * (long long)a.c.capacity;
-  int32_t* positions_out = a.positions_out + bh * (long long)a.c.capacity;
-  const long long border = (long long)a.next[b] - a.recent;
-  auto key = [&](int i) -> unsigned {
-    const long long p = positions[i];
-    return p < a.sinks || p >= border ? 0x80000000u : (unsigned)max(scores[i], 0);
-  };
+  const size_t base = (size_t)bh * a.c.capacity;
+  const int32_t* scores = a.c.scores + base;
+  const int32_t* positions = a.c.positions + base;
+  int32_t* scores_out = a.scores_out + base;
+  int32_t* positions_out = a.positions_out + base;
   if (n <= keep) {
     for (int i = tid; i < n; i += SEL_THREADS) {
       scores_out[i] = scores[i];
@@ -216,130 +220,238 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
     if (tid == 0) a.moves[bh] = 0;
     return;
   }
-  // ---- the keep-th largest key ----
-  unsigned prefix = 0;
-  int want = keep;  // how many of the keys that share the prefix stay
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += SEL_THREADS) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += SEL_THREADS) {
-      const unsigned k = key(i);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
-    }
-    __syncthreads();
-    if (warp == 0) {
-      // lane l holds bins 255 - 8 l down to 248 - 8 l: a scan from the top
-      int own[8], sum = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        own[j] = hist[255 - 8 * lane - j];
-        sum += own[j];
-      }
-      int before = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
-      }
-      before -= sum;  // keys in higher bins of other lanes
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (before < want && before + own[j] >= want) {
-          s_prefix = prefix | (unsigned)(255 - 8 * lane - j) << shift;
-          s_want = want - before;
-        }
-        before += own[j];
-      }
-    }
-    __syncthreads();
-    prefix = s_prefix;
-    want = s_want;
-    __syncthreads();
-  }
-  const unsigned border_key = prefix;  // keys above it stay, and the first `want` slots that equal it
-
+  const long long border = (long long)a.next[b] - a.recent;
   // Each warp takes one contiguous span of slots, 32 at a time, so that ranks
   // follow the slot order.
   const int span = ((n + SEL_WARPS - 1) / SEL_WARPS + 31) / 32 * 32;
   const int lo = min(n, warp * span), hi = min(n, lo + span);
-  auto prefix_of_warps = [&](int* mine) {  // exclusive prefix of warp counts; all threads
-    __syncthreads();
+  const int rounds = (hi - lo + 31) / 32;
+  auto key_of = [&](int i) -> unsigned {
+    const long long p = positions[i];
+    return p < a.sinks || p >= border ? SAFE : (unsigned)max(scores[i], 0);
+  };
+  unsigned held[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    const int i = lo + 32 * k + lane;
+    held[k] = i < hi ? key_of(i) : NONE;
+  }
+  // f(round, key) for every round of the warp's span; lanes past it get NONE
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+      if (k < rounds) f(k, held[k]);
+    for (int k = HELD; k < rounds; ++k) {
+      const int i = lo + 32 * k + lane;
+      f(k, i < hi ? key_of(i) : NONE);
+    }
+  };
+
+  // ---- the protected slots, and the largest other key ----
+  int safe = 0;
+  unsigned top = 0;
+  each([&](int, unsigned k) {
+    safe += k == SAFE;
+    top = max(top, k < SAFE ? k : 0u);
+  });
+  safe = __reduce_add_sync(0xffffffffu, safe);
+  top = __reduce_max_sync(0xffffffffu, top);
+  __syncthreads();
+  if (lane == 0) {
+    atomicAdd(&s_safe, safe);
+    atomicMax(&s_top, top);
+  }
+  __syncthreads();
+  // ---- the last key that stays: kept are the keys above it, and the first `want` slots that equal it ----
+  unsigned last = SAFE;
+  int want = keep;
+  if (s_safe < keep) {
+    want = keep - s_safe;
+    unsigned prefix = 0;
+    int shift = s_top == 0 ? 0 : max(0, 24 - __clz(s_top));  // the top eight bits in use first
+    int fixed = 31;  // the bits of `prefix` from here up are settled
+    for (;;) {
+      for (int i = tid; i < 256; i += SEL_THREADS) hist[i] = 0;
+      __syncthreads();
+      each([&](int, unsigned k) {
+        if (k < SAFE && (k >> fixed) == (prefix >> fixed)) atomicAdd(&hist[(k >> shift) & 255], 1);
+      });
+      __syncthreads();
+      if (warp == 0) {
+        // lane l holds bins 255 - 8 l down to 248 - 8 l: a scan from the top
+        int own[8], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          own[j] = hist[255 - 8 * lane - j];
+          sum += own[j];
+        }
+        int before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += v;
+        }
+        before -= sum;  // keys in higher bins of other lanes
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (before < want && before + own[j] >= want) {
+            s_prefix = (prefix & ~(255u << shift)) | (unsigned)(255 - 8 * lane - j) << shift;
+            s_want = want - before;
+            s_top = (unsigned)own[j];
+          }
+          before += own[j];
+        }
+      }
+      __syncthreads();
+      prefix = s_prefix;
+      want = s_want;
+      const bool all = want == (int)s_top;  // every key of the bin stays: what lies above prefix - 1
+      __syncthreads();
+      if (all && prefix > 0) {
+        last = prefix - 1;
+        want = 0;
+        break;
+      }
+      if (shift == 0) {
+        last = prefix;
+        break;
+      }
+      fixed = shift;
+      shift = max(0, shift - 8);
+    }
+  }
+
+  auto prefix_of_warps = [&](const int* mine) {  // exclusive prefix of warp counts
     int s = 0;
     for (int w = 0; w < warp; ++w) s += mine[w];
     return s;
   };
-  int equal = 0;
-  for (int i = lo + lane; i - lane < hi; i += 32) equal += __popc(__ballot_sync(0xffffffffu, i < hi && key(i) == border_key));
-  if (lane == 0) warp_a[warp] = equal;
-  int rank = prefix_of_warps(warp_a);
-  int holes = 0, late = 0;
-  for (int i = lo + lane; i - lane < hi; i += 32) {
-    const unsigned k = i < hi ? key(i) : 0u;
-    const unsigned eq = __ballot_sync(0xffffffffu, i < hi && k == border_key);
-    const bool kept = i < hi && (k > border_key || (k == border_key && rank + __popc(eq & ((1u << lane) - 1)) < want));
-    rank += __popc(eq);
-    const unsigned kept_bits = __ballot_sync(0xffffffffu, kept);
-    holes += __popc(__ballot_sync(0xffffffffu, i < hi && i < keep && !kept));
-    late += __popc(__ballot_sync(0xffffffffu, kept && i >= keep));
-    if (lane == 0) bitmap[i >> 5] = kept_bits;  // spans are multiples of 32 slots
-    if (kept && i < keep) {
-      scores_out[i] = scores[i];
-      positions_out[i] = positions[i];
-    }
+  int rank = 0;
+  if (want > 0) {  // ties go to the lower slots
+    int equal = 0;
+    each([&](int, unsigned k) { equal += k == last; });
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if (lane == 0) warp_a[warp] = equal;
+    __syncthreads();
+    rank = prefix_of_warps(warp_a);
+    __syncthreads();
   }
-  __syncthreads();
+  const unsigned under = (1u << lane) - 1;
+  int holes = 0, late = 0;
+  each([&](int r, unsigned k) {
+    const int i = lo + 32 * r + lane;
+    bool kept = k != NONE && k > last;
+    if (want > 0) {
+      const unsigned eq = __ballot_sync(0xffffffffu, k == last);
+      kept = kept || (k == last && rank + __popc(eq & under) < want);
+      rank += __popc(eq);
+    }
+    const unsigned bits = __ballot_sync(0xffffffffu, kept);
+    if (lane == 0) bitmap[(lo >> 5) + r] = bits;
+    // of the round's slots, those below `keep`
+    const int low = max(0, min(32, keep - (lo + 32 * r))), live = min(32, hi - (lo + 32 * r));
+    const unsigned low_mask = low >= 32 ? 0xffffffffu : (1u << low) - 1;
+    const unsigned live_mask = live >= 32 ? 0xffffffffu : (1u << live) - 1;
+    holes += __popc(~bits & low_mask & live_mask);
+    late += __popc(bits & ~low_mask);
+    if (kept && i < keep && scores_out != scores) scores_out[i] = scores[i];
+    if (kept && i < keep && positions_out != positions) positions_out[i] = positions[i];
+  });
   if (lane == 0) {
     warp_a[warp] = holes;
     warp_b[warp] = late;
   }
+  __syncthreads();
   int hole_rank = prefix_of_warps(warp_a), late_rank = prefix_of_warps(warp_b);
-  int2* list = a.list + bh * a.most;
-  for (int i = lo + lane; i - lane < hi; i += 32) {
-    const bool kept = (bitmap[i >> 5] >> lane) & 1;
+  int2* list = a.list + (size_t)bh * a.most;
+  for (int r = 0; r < rounds; ++r) {
+    const int i = lo + 32 * r + lane;
+    const unsigned bits = bitmap[(lo >> 5) + r];
+    const bool kept = (bits >> lane) & 1;
     const bool hole = i < hi && i < keep && !kept, moves = i < hi && i >= keep && kept;
     const unsigned hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, moves);
-    const unsigned below = (1u << lane) - 1;
-    if (hole) list[hole_rank + __popc(hb & below)].y = i;
-    if (moves) list[late_rank + __popc(mb & below)].x = i;
+    if (hole) list[hole_rank + __popc(hb & under)].y = i;
+    if (moves) list[late_rank + __popc(mb & under)].x = i;
     hole_rank += __popc(hb);
     late_rank += __popc(mb);
   }
   if (tid == SEL_THREADS - 1) a.moves[bh] = late_rank;  // the last warp's running rank is the total
 }
 
-// One warp per move: the slot's codes, scales, score and position as 4-byte words.
+// A move is 2 head_dim / 2 code bytes, the scales, the score and the position:
+// 88 bytes at 64 dims, in pieces of 16, 8 and 4 bytes, one a lane, LANES lanes
+// a move, and UNROLL moves of a lane in flight.
+template <int HD>
 __global__ void __launch_bounds__(THREADS) q4_move_kernel(const EvictArgs a) {
+  constexpr int LANES = HD == 256 ? 32 : 8, UNROLL = 4, PER = THREADS / LANES;
+  constexpr int CODE = HD / 2;                         // bytes of a slot's codes in one tensor
+  constexpr int SCALE = HD < 32 ? 4 : HD / 8;          // and of its scales
+  constexpr int CB = CODE < 16 ? CODE : 16, SB = SCALE < 16 ? SCALE : 16;  // piece sizes
+  constexpr int CN = CODE / CB, SN = SCALE / SB;       // pieces
+  static_assert(2 * CN + 2 * SN + 2 <= LANES);
   griddep_wait();
   griddep_launch();
-  const long long bh = blockIdx.x;
+  const unsigned bh = blockIdx.x;
   const int moves = a.moves[bh];
-  const int cw = (int)a.c.head_dim / 8, gw = a.c.head_dim < 32 ? 1 : (int)a.c.head_dim / 32;
-  const int words = 2 * cw + 2 * gw + 2;
-  const int lane = threadIdx.x & 31;
   const size_t base = (size_t)bh * a.c.capacity;
-  uint32_t* kc = reinterpret_cast<uint32_t*>(a.c.k_codes);
-  uint32_t* vc = reinterpret_cast<uint32_t*>(a.c.v_codes);
-  for (int m = blockIdx.y * (THREADS / 32) + (threadIdx.x >> 5); m < moves; m += gridDim.y * (THREADS / 32)) {
-    const int2 e = a.list[bh * a.most + m];
-    const size_t from = base + (size_t)e.x, to = base + (size_t)e.y;
-    for (int w = lane; w < words; w += 32) {
-      if (w < cw)
-        kc[to * cw + w] = kc[from * cw + w];
-      else if (w < 2 * cw)
-        vc[to * cw + w - cw] = vc[from * cw + w - cw];
-      else if (w < 2 * cw + gw)
-        a.c.k_scales[to * gw + w - 2 * cw] = a.c.k_scales[from * gw + w - 2 * cw];
-      else if (w < 2 * cw + 2 * gw)
-        a.c.v_scales[to * gw + w - 2 * cw - gw] = a.c.v_scales[from * gw + w - 2 * cw - gw];
-      else if (w == words - 2)
-        a.scores_out[to] = a.c.scores[from];
+  // this lane's piece: where it comes from, where it goes, bytes, stride of a slot
+  const int piece = threadIdx.x % LANES;
+  const uint8_t* src = nullptr;
+  uint8_t* dst = nullptr;
+  int bytes = 0, stride = 0;
+  auto take = [&](const void* from, void* to, int size, int slot_bytes, int offset) {
+    src = static_cast<const uint8_t*>(from) + base * slot_bytes + offset;
+    dst = static_cast<uint8_t*>(to) + base * slot_bytes + offset;
+    bytes = size;
+    stride = slot_bytes;
+  };
+  if (piece < CN)
+    take(a.c.k_codes, a.c.k_codes, CB, CODE, CB * piece);
+  else if (piece < 2 * CN)
+    take(a.c.v_codes, a.c.v_codes, CB, CODE, CB * (piece - CN));
+  else if (piece < 2 * CN + SN)
+    take(a.c.k_scales, a.c.k_scales, SB, SCALE, SB * (piece - 2 * CN));
+  else if (piece < 2 * CN + 2 * SN)
+    take(a.c.v_scales, a.c.v_scales, SB, SCALE, SB * (piece - 2 * CN - SN));
+  else if (piece == 2 * CN + 2 * SN)
+    take(a.c.scores, a.scores_out, 4, 4, 0);
+  else if (piece == 2 * CN + 2 * SN + 1)
+    take(a.c.positions, a.positions_out, 4, 4, 0);
+  const int2* list = a.list + (size_t)bh * a.most;
+  for (int m0 = blockIdx.y * PER * UNROLL; m0 < moves; m0 += gridDim.y * PER * UNROLL) {
+    int2 e[UNROLL];
+    uint4 v[UNROLL];
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      const int m = m0 + k * PER + threadIdx.x / LANES;
+      e[k] = m < moves && bytes ? list[m] : make_int2(-1, -1);
+    }
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      if (e[k].x < 0) continue;
+      const uint8_t* s = src + (size_t)e[k].x * stride;
+      if (bytes == 16)
+        v[k] = *reinterpret_cast<const uint4*>(s);
+      else if (bytes == 8)
+        *reinterpret_cast<uint2*>(&v[k]) = *reinterpret_cast<const uint2*>(s);
       else
-        a.positions_out[to] = a.c.positions[from];
+        v[k].x = *reinterpret_cast<const uint32_t*>(s);
+    }
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      if (e[k].x < 0) continue;
+      uint8_t* d = dst + (size_t)e[k].y * stride;
+      if (bytes == 16)
+        *reinterpret_cast<uint4*>(d) = v[k];
+      else if (bytes == 8)
+        *reinterpret_cast<uint2*>(d) = make_uint2(v[k].x, v[k].y);
+      else
+        *reinterpret_cast<uint32_t*>(d) = v[k].x;
     }
   }
   // lens_out may be lens, so it changes only after the selection has read it
-  if (blockIdx.y == 0 && bh % (long long)a.c.heads == 0 && threadIdx.x == 0) {
-    const long long b = bh / (long long)a.c.heads;
+  if (blockIdx.y == 0 && bh % (unsigned)a.c.heads == 0 && threadIdx.x == 0) {
+    const unsigned b = bh / (unsigned)a.c.heads;
     const int n = a.lens[b];
     if (n >= 0 && n <= (int)a.c.capacity) a.lens_out[b] = min(n, (int)a.keep);
   }
@@ -348,35 +460,33 @@ __global__ void __launch_bounds__(THREADS) q4_move_kernel(const EvictArgs a) {
 size_t most_moves(const nsrl_q4_cache& c, size_t keep) { return std::min(keep, c.capacity - keep); }
 size_t list_offset(const nsrl_q4_cache& c) { return (c.batch * c.heads * sizeof(int32_t) + 255) & ~size_t(255); }
 
-unsigned blocks_for(long long threads) { return (unsigned)((threads + THREADS - 1) / THREADS); }
-
 }  // namespace
 
 cudaError_t launch_q4_append(const nsrl_q4_cache& c, const int16_t* k, const int16_t* v, size_t ld, size_t tokens,
                              const int32_t* starts, const int32_t* counts, const int32_t* positions,
                              nsrl_device_status* st, cudaStream_t s) {
-  const long long threads = (long long)(c.batch * c.heads * tokens * (c.head_dim / 8));
-  if (threads == 0) return cudaSuccess;
-  if (threads > (long long)THREADS * 0x7fffffffll) return cudaErrorInvalidValue;
-  const AppendArgs a{c, k, v, (long long)ld, (long long)tokens, starts, counts, positions, st};
+  const size_t n = c.batch * c.heads * tokens, per_block = THREADS / (c.head_dim / 8);
+  if (n == 0) return cudaSuccess;
+  if (n > 0xffffff00u) return cudaErrorInvalidValue;  // the entry point refuses it
+  const AppendArgs a{c, k, v, (long long)ld, (long long)tokens, (unsigned)n, starts, counts, positions, st};
   const bool vec = ld % 8 == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
   const double rows = (double)(c.batch * c.heads) * (double)tokens;
   ProfScope prof("q4_append", s, 0.0, rows * (4.0 * c.head_dim + c.head_dim + 8.0 * std::max<size_t>(1, c.head_dim / 32)));
   auto* kernel = c.head_dim == 16 ? q4_append_kernel<16> : c.head_dim == 64 ? q4_append_kernel<64> : q4_append_kernel<256>;
-  const cudaError_t e = launch_pdl(kernel, dim3(blocks_for(threads)), dim3(THREADS), 0, s, a, vec);
+  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)((n + per_block - 1) / per_block)), dim3(THREADS), 0, s, a, vec);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 cudaError_t launch_q4_read(const nsrl_q4_cache& c, const int32_t* starts, size_t tokens, int16_t* k, int16_t* v,
                            nsrl_device_status* st, cudaStream_t s) {
-  const long long threads = (long long)(c.batch * c.heads * tokens * (c.head_dim / 8));
-  if (threads == 0) return cudaSuccess;
-  if (threads > (long long)THREADS * 0x7fffffffll) return cudaErrorInvalidValue;
-  const ReadArgs a{c, starts, (long long)tokens, k, v, st};
+  const size_t n = c.batch * c.heads * tokens, per_block = THREADS / (c.head_dim / 8);
+  if (n == 0) return cudaSuccess;
+  if (n > 0xffffff00u) return cudaErrorInvalidValue;  // the entry point refuses it
+  const ReadArgs a{c, starts, (long long)tokens, (unsigned)n, k, v, st};
   const double rows = (double)(c.batch * c.heads) * (double)tokens;
   ProfScope prof("q4_read", s, 0.0, rows * (4.0 * c.head_dim + c.head_dim + 8.0 * std::max<size_t>(1, c.head_dim / 32)));
   auto* kernel = c.head_dim == 16 ? q4_read_kernel<16> : c.head_dim == 64 ? q4_read_kernel<64> : q4_read_kernel<256>;
-  const cudaError_t e = launch_pdl(kernel, dim3(blocks_for(threads)), dim3(THREADS), 0, s, a);
+  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)((n + per_block - 1) / per_block)), dim3(THREADS), 0, s, a);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -405,14 +515,26 @@ cudaError_t launch_q4_evict(const nsrl_q4_cache& c, const int32_t* lens, const i
   a.st = st;
   const size_t smem = (c.capacity / 32 + 1) * sizeof(uint32_t);
   {
+    // Threads and keys a thread holds follow the capacity: up to 8,192 slots in
+    // 256 threads (several CTAs an SM hide each other's barriers: 2,048 rows of
+    // 2,112 slots took 96 us in 1,024 threads that read their keys again each
+    // pass), above that 1,024 threads.
+    auto* kernel = c.capacity <= 2048   ? q4_select_kernel<256, 8>
+                   : c.capacity <= 4096 ? q4_select_kernel<256, 16>
+                   : c.capacity <= 8192 ? q4_select_kernel<256, 32>
+                                        : q4_select_kernel<1024, 32>;
     ProfScope prof("q4_select", s, 0.0, 8.0 * (double)bh * (double)c.capacity);
-    cudaError_t e = cudaFuncSetAttribute(q4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = launch_pdl(q4_select_kernel, dim3((unsigned)bh), dim3(SEL_THREADS), smem, s, a);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess)
+      e = launch_pdl(kernel, dim3((unsigned)bh), dim3(c.capacity <= 8192 ? 256 : 1024), smem, s, a);
     if (e != cudaSuccess) return e;
   }
-  const unsigned chunks = (unsigned)std::max<size_t>(1, std::min<size_t>((a.most + 63) / 64, 64));
+  // moves of a CTA's step: 128 (32 at 256 dims), as many CTAs a row as its moves may need, 64 at most
+  const size_t step = c.head_dim == 256 ? 32 : 128;
+  const unsigned chunks = (unsigned)std::max<size_t>(1, std::min<size_t>((a.most + step - 1) / step, 64));
   ProfScope prof("q4_move", s, 0.0, 2.0 * (double)bh * (double)a.most * (double)c.head_dim);
-  const cudaError_t e = launch_pdl(q4_move_kernel, dim3((unsigned)bh, chunks), dim3(THREADS), 0, s, a);
+  auto* kernel = c.head_dim == 16 ? q4_move_kernel<16> : c.head_dim == 64 ? q4_move_kernel<64> : q4_move_kernel<256>;
+  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)bh, chunks), dim3(THREADS), 0, s, a);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -32,7 +32,7 @@ struct RotArgs {
   long long ldx, ldy, rows;
   const unsigned long long* turns;
   const int32_t* positions;
-  long long seq_len;
+  unsigned seq_len;
   int heads, hd, half, interleaved, backward, amplitude;
   int block_rows;
 };
@@ -84,65 +84,97 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
   const int per_head = turning + passing, per_row = per_head * a.heads;
   const int items = rows * per_row;
 
-  // element offsets of an item's two accesses within its row, and its first pair
-  auto place = [&](int it, int& row, int& i0, int& i1, int& pair) {
-    row = it / per_row;
-    const int in_row = it - row * per_row;
-    const int head = in_row / per_head, slot = in_row - head * per_head;
-    const int base = head * a.hd;
-    if (slot < turning) {
-      pair = VEC ? 8 * slot : slot;
+  // An item's place, stepped from one to the next by THREADS in mixed radix:
+  // two divisions a thread instead of two an item.
+  struct Place {
+    int row, head, slot;
+  };
+  const int step_row = THREADS / per_row, step_head = THREADS % per_row / per_head, step_slot = THREADS % per_head;
+  auto next = [&](Place& p) {
+    p.slot += step_slot;
+    p.head += step_head;
+    p.row += step_row;
+    if (p.slot >= per_head) {
+      p.slot -= per_head;
+      ++p.head;
+    }
+    if (p.head >= a.heads) {
+      p.head -= a.heads;
+      ++p.row;
+    }
+  };
+  // element offsets of an item's two accesses within its row, and its first pair (-1: passes through)
+  auto offsets = [&](const Place& p, int& i0, int& i1) -> int {
+    const int base = p.head * a.hd;
+    if (p.slot < turning) {
+      const int pair = VEC ? 8 * p.slot : p.slot;
       i0 = base + (a.interleaved ? 2 * pair : pair);
       i1 = a.interleaved ? i0 + (VEC ? 8 : 1) : i0 + a.half;
-    } else {
-      pair = -1;
-      i0 = base + 2 * a.half + (VEC ? 16 : 1) * (slot - turning);
-      i1 = i0 + (VEC ? 8 : 0);
+      return pair;
     }
+    i0 = base + 2 * a.half + (VEC ? 16 : 1) * (p.slot - turning);
+    i1 = i0 + (VEC ? 8 : 0);
+    return -1;
   };
 
   griddep_wait();
   griddep_launch();
   uint4 v0[ITEMS], v1[ITEMS];
-  auto load = [&](int it, uint4& u0, uint4& u1) {
-    int row, i0, i1, pair;
-    place(it, row, i0, i1, pair);
-    const int16_t* p = a.x + (row0 + row) * a.ldx;
+  auto load = [&](const Place& p, uint4& u0, uint4& u1) {
+    int i0, i1;
+    offsets(p, i0, i1);
+    const int16_t* x = a.x + (row0 + p.row) * a.ldx;
     if (VEC) {
-      u0 = *reinterpret_cast<const uint4*>(p + i0);
-      u1 = *reinterpret_cast<const uint4*>(p + i1);
+      u0 = *reinterpret_cast<const uint4*>(x + i0);
+      u1 = *reinterpret_cast<const uint4*>(x + i1);
     } else {
-      u0.x = (uint32_t)(uint16_t)p[i0];
-      u1.x = (uint32_t)(uint16_t)p[i1];
+      u0.x = (uint32_t)(uint16_t)x[i0];
+      u1.x = (uint32_t)(uint16_t)x[i1];
     }
   };
+  Place start;
+  start.row = threadIdx.x / per_row;
+  start.head = threadIdx.x % per_row / per_head;
+  start.slot = threadIdx.x % per_head;
+  Place at = start;
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int it = threadIdx.x + k * THREADS;
-    if (it < items) load(it, v0[k], v1[k]);
+    if (threadIdx.x + k * THREADS < items) load(at, v0[k], v1[k]);
+    next(at);
   }
-  for (int i = threadIdx.x; i < rows * a.half; i += THREADS) {
-    const int row = i / a.half, pair = i - row * a.half;
-    const long long r = row0 + row;
-    const long long p = a.positions ? (long long)a.positions[r] : r % a.seq_len;
-    int c, s;
-    cos_sin_q30((unsigned long long)p * a.turns[pair], a.amplitude, c, s);
-    sc[i] = c;
-    ss[i] = a.backward ? -s : s;
+  {
+    int row = threadIdx.x / a.half, pair = threadIdx.x % a.half;
+    const int down = THREADS / a.half, along = THREADS % a.half;
+    for (int i = threadIdx.x; i < rows * a.half; i += THREADS) {
+      const long long r = row0 + row;
+      const long long p = a.positions ? (long long)a.positions[r] : (long long)((unsigned)r % a.seq_len);
+      int c, s;
+      cos_sin_q30((unsigned long long)p * a.turns[pair], a.amplitude, c, s);
+      sc[i] = c;
+      ss[i] = a.backward ? -s : s;
+      row += down;
+      pair += along;
+      if (pair >= a.half) {
+        pair -= a.half;
+        ++row;
+      }
+    }
   }
   __syncthreads();
 
+  at = start;
   for (int it0 = threadIdx.x; it0 < items; it0 += ITEMS * THREADS) {
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      const int it = it0 + k * THREADS;
-      if (it >= items) continue;
-      if (it0 >= ITEMS * THREADS) load(it, v0[k], v1[k]);  // past the items loaded ahead
-      int row, i0, i1, pair;
-      place(it, row, i0, i1, pair);
-      int16_t* p = a.y + (row0 + row) * a.ldy;
-      const int32_t* c = sc + row * a.half + pair;
-      const int32_t* s = ss + row * a.half + pair;
+      const Place here = at;
+      next(at);
+      if (it0 + k * THREADS >= items) continue;
+      if (it0 >= ITEMS * THREADS) load(here, v0[k], v1[k]);  // past the items loaded ahead
+      int i0, i1;
+      const int pair = offsets(here, i0, i1);
+      int16_t* p = a.y + (row0 + here.row) * a.ldy;
+      const int32_t* c = sc + here.row * a.half + pair;
+      const int32_t* s = ss + here.row * a.half + pair;
       if (VEC) {
         uint4 o0 = v0[k], o1 = v1[k];
         if (pair >= 0) {
@@ -196,7 +228,7 @@ cudaError_t launch_rotary(const int16_t* x, size_t rows, size_t heads, size_t hd
   a.rows = (long long)rows;
   a.turns = reinterpret_cast<const unsigned long long*>(rot.turns);
   a.positions = positions;
-  a.seq_len = (long long)seq_len;
+  a.seq_len = (unsigned)std::min<size_t>(std::max<size_t>(seq_len, 1), 0x7fffffff);
   a.heads = (int)heads;
   a.hd = (int)hd;
   a.half = (int)(rot.rotary_dim / 2);
