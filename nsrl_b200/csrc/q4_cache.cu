@@ -41,30 +41,28 @@ __device__ __forceinline__ uint4 load8(const int16_t* p, bool vec) {
 // Eight dims to eight codes; scale_word is the group's (LPG lanes of the warp).
 template <int LPG>
 __device__ __forceinline__ uint32_t quantise8(const uint4& u, uint32_t& scale_word) {
-  int x[8];
-  unpack8(u, x);
-  int lo = x[0], hi = x[0];
+  // smallest values and smallest complements (so the largest values), two at a time
+  uint32_t low = __vmins2(__vmins2(u.x, u.y), __vmins2(u.z, u.w));
+  uint32_t high = __vmaxs2(__vmaxs2(u.x, u.y), __vmaxs2(u.z, u.w));
+  uint32_t both = __vmins2(__byte_perm(low, ~high, 0x5410), __byte_perm(low, ~high, 0x7632));
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min(lo, x[i]);
-    hi = max(hi, x[i]);
-  }
-#pragma unroll
-  for (int o = 1; o < LPG; o <<= 1) {
-    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
+  for (int o = 1; o < LPG; o <<= 1) both = __vmins2(both, __shfl_xor_sync(0xffffffffu, both, o));
+  const int lo = (int)(int16_t)(both & 0xFFFF), hi = ~((int)both >> 16);
   const unsigned scale = max(1u, (unsigned)(hi - lo + 14) / 15u);
   // floor(n / d) = n * ceil(2^32 / d) >> 32 while n d < 2^32 (Granlund and
   // Montgomery): n = 2 (x - lo) + scale < 2^17.1, d = 2 scale < 2^13.1
   const unsigned d = 2 * scale;
   const unsigned magic = 0xFFFFFFFFu / d + 1;
+  const int offset = (int)scale - 2 * lo;
+  const bool top = hi + (int)(scale / 2) > 32767;  // a value may pass 32767
+  int x[8];
+  unpack8(u, x);
   uint32_t codes = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    int q = (int)__umulhi(2u * (unsigned)(x[i] - lo) + scale, magic);
-    q -= lo + (int)scale * q > 32767 ? 1 : 0;
-    codes |= (uint32_t)q << (4 * i);
+  for (int i = 7; i >= 0; --i) {
+    int q = (int)__umulhi((unsigned)(2 * x[i] + offset), magic);
+    if (top) q -= lo + (int)scale * q > 32767 ? 1 : 0;
+    codes = codes * 16 + (uint32_t)q;
   }
   scale_word = scale | ((uint32_t)lo << 16);
   return codes;
@@ -87,6 +85,7 @@ __global__ void __launch_bounds__(THREADS) q4_append_kernel(const AppendArgs a, 
   const bool fits = start >= 0 && count >= 0 && count <= a.tokens && start + count <= (long long)a.c.capacity;
   if (inside && !fits && t == 0 && sub == 0 && h == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
   const bool live = inside && fits && (long long)t < count;
+  if (!__any_sync(0xffffffffu, live)) return;
   uint4 uk = make_uint4(0, 0, 0, 0), uv = uk;
   if (live) {
     const long long off = ((long long)b * a.tokens + t) * a.ld + (long long)h * HD + 8 * sub;
@@ -179,9 +178,9 @@ struct EvictArgs {
   nsrl_device_status* st;
 };
 
-// The first keys of a thread's span stay in registers (HELD of them, chosen from
-// the capacity); a longer span's others are read again in each pass.  Bound by
-// memory: 8 bytes a slot in, 8 a kept slot out.
+// The first HELD slots of a thread's span stay in registers (loaded all at once:
+// the loads' latency is most of a short row's time); a longer span's others are
+// read again in each pass.  Bound by memory: 8 bytes a slot in, 8 a kept slot out.
 template <int SEL_THREADS, int HELD>
 __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs a) {
   constexpr int SEL_WARPS = SEL_THREADS / 32;
@@ -226,31 +225,35 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
   const int span = ((n + SEL_WARPS - 1) / SEL_WARPS + 31) / 32 * 32;
   const int lo = min(n, warp * span), hi = min(n, lo + span);
   const int rounds = (hi - lo + 31) / 32;
-  auto key_of = [&](int i) -> unsigned {
-    const long long p = positions[i];
-    return p < a.sinks || p >= border ? SAFE : (unsigned)max(scores[i], 0);
+  auto key_of = [&](int score, int position) -> unsigned {
+    return (long long)position < a.sinks || (long long)position >= border ? SAFE : (unsigned)max(score, 0);
   };
-  unsigned held[HELD];
+  int score[HELD], position[HELD];
+  unsigned key[HELD];
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     const int i = lo + 32 * k + lane;
-    held[k] = i < hi ? key_of(i) : NONE;
+    score[k] = i < hi ? scores[i] : 0;
+    position[k] = i < hi ? positions[i] : 0;
   }
-  // f(round, key) for every round of the warp's span; lanes past it get NONE
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) key[k] = lo + 32 * k + lane < hi ? key_of(score[k], position[k]) : NONE;
+  // f(round, key, score, position) for every round of the warp's span; lanes past it get NONE
   auto each = [&](auto f) {
 #pragma unroll
     for (int k = 0; k < HELD; ++k)
-      if (k < rounds) f(k, held[k]);
+      if (k < rounds) f(k, key[k], score[k], position[k]);
     for (int k = HELD; k < rounds; ++k) {
       const int i = lo + 32 * k + lane;
-      f(k, i < hi ? key_of(i) : NONE);
+      const int s = i < hi ? scores[i] : 0, p = i < hi ? positions[i] : 0;
+      f(k, i < hi ? key_of(s, p) : NONE, s, p);
     }
   };
 
   // ---- the protected slots, and the largest other key ----
   int safe = 0;
   unsigned top = 0;
-  each([&](int, unsigned k) {
+  each([&](int, unsigned k, int, int) {
     safe += k == SAFE;
     top = max(top, k < SAFE ? k : 0u);
   });
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
     for (;;) {
       for (int i = tid; i < 256; i += SEL_THREADS) hist[i] = 0;
       __syncthreads();
-      each([&](int, unsigned k) {
+      each([&](int, unsigned k, int, int) {
         if (k < SAFE && (k >> fixed) == (prefix >> fixed)) atomicAdd(&hist[(k >> shift) & 255], 1);
       });
       __syncthreads();
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
   int rank = 0;
   if (want > 0) {  // ties go to the lower slots
     int equal = 0;
-    each([&](int, unsigned k) { equal += k == last; });
+    each([&](int, unsigned k, int, int) { equal += k == last; });
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) warp_a[warp] = equal;
     __syncthreads();
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
   }
   const unsigned under = (1u << lane) - 1;
   int holes = 0, late = 0;
-  each([&](int r, unsigned k) {
+  each([&](int r, unsigned k, int s, int p) {
     const int i = lo + 32 * r + lane;
     bool kept = k != NONE && k > last;
     if (want > 0) {
@@ -354,8 +357,10 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
     const unsigned live_mask = live >= 32 ? 0xffffffffu : (1u << live) - 1;
     holes += __popc(~bits & low_mask & live_mask);
     late += __popc(bits & ~low_mask);
-    if (kept && i < keep && scores_out != scores) scores_out[i] = scores[i];
-    if (kept && i < keep && positions_out != positions) positions_out[i] = positions[i];
+    if (kept && i < keep) {
+      if (scores_out != scores) scores_out[i] = s;
+      if (positions_out != positions) positions_out[i] = p;
+    }
   });
   if (lane == 0) {
     warp_a[warp] = holes;
@@ -515,18 +520,18 @@ cudaError_t launch_q4_evict(const nsrl_q4_cache& c, const int32_t* lens, const i
   a.st = st;
   const size_t smem = (c.capacity / 32 + 1) * sizeof(uint32_t);
   {
-    // Threads and keys a thread holds follow the capacity: up to 8,192 slots in
-    // 256 threads (several CTAs an SM hide each other's barriers: 2,048 rows of
-    // 2,112 slots took 96 us in 1,024 threads that read their keys again each
-    // pass), above that 1,024 threads.
-    auto* kernel = c.capacity <= 2048   ? q4_select_kernel<256, 8>
-                   : c.capacity <= 4096 ? q4_select_kernel<256, 16>
-                   : c.capacity <= 8192 ? q4_select_kernel<256, 32>
-                                        : q4_select_kernel<1024, 32>;
+    // Threads follow the capacity, 16 slots a thread up to 16,384: several CTAs an
+    // SM hide each other's barriers (2,048 rows of 2,112 slots took 96 us in 1,024
+    // threads that read their keys again each pass).
+    const unsigned threads = c.capacity <= 2048 ? 128 : c.capacity <= 4096 ? 256 : c.capacity <= 8192 ? 512 : 1024;
+    auto* kernel = threads == 128   ? q4_select_kernel<128, 16>
+                   : threads == 256 ? q4_select_kernel<256, 16>
+                   : threads == 512 ? q4_select_kernel<512, 16>
+                                    : q4_select_kernel<1024, 16>;
     ProfScope prof("q4_select", s, 0.0, 8.0 * (double)bh * (double)c.capacity);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess)
-      e = launch_pdl(kernel, dim3((unsigned)bh), dim3(c.capacity <= 8192 ? 256 : 1024), smem, s, a);
+      e = launch_pdl(kernel, dim3((unsigned)bh), dim3(threads), smem, s, a);
     if (e != cudaSuccess) return e;
   }
   // moves of a CTA's step: 128 (32 at 256 dims), as many CTAs a row as its moves may need, 64 at most

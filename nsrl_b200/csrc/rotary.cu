@@ -33,7 +33,7 @@ struct RotArgs {
   const unsigned long long* turns;
   const int32_t* positions;
   unsigned seq_len;
-  int heads, hd, half, interleaved, backward, amplitude;
+  int heads, hd, half, backward, amplitude;
   int block_rows;
 };
 
@@ -50,28 +50,26 @@ __device__ __forceinline__ void cos_sin_q30(unsigned long long a, int amplitude,
     C0 = -C0;
   }
   const int r = __mulhi((int)(d >> 22), 1686629713);
-  const int h = (__mulhi(r, r) + (1 << 14)) >> 15;
-  const long long h256 = (long long)h << 8, half = 1ll << 37;
-  long long cc = C0 - ((C0 * h256 + (long long)S0 * r + half) >> 38);
-  long long ss = S0 - ((S0 * h256 - (long long)C0 * r + half) >> 38);
+  const int h256 = ((__mulhi(r, r) + (1 << 14)) >> 15) << 8;  // below 2^21
+  const long long half = 1ll << 37;
+  c = C0 - (int)(((long long)C0 * h256 + (long long)S0 * r + half) >> 38);
+  s = S0 - (int)(((long long)S0 * h256 - (long long)C0 * r + half) >> 38);
   if (amplitude != (1 << 30)) {
-    cc = (cc * amplitude + (1ll << 29)) >> 30;
-    ss = (ss * amplitude + (1ll << 29)) >> 30;
+    // |c| may pass 2^30 by one, so an amplitude near 2 may reach 2^31: held to 2^31 - 1
+    c = (int)max(-2147483647ll, min(2147483647ll, ((long long)c * amplitude + (1ll << 29)) >> 30));
+    s = (int)max(-2147483647ll, min(2147483647ll, ((long long)s * amplitude + (1ll << 29)) >> 30));
   }
-  // |C| may pass 2^30 by one, so an amplitude near 2 may reach 2^31: held to 2^31 - 1
-  c = (int)max(-2147483647ll, min(2147483647ll, cc));
-  s = (int)max(-2147483647ll, min(2147483647ll, ss));
 }
 
-// rhu(x0 * c + x1 * s, 30), saturated; the sum stays below 2^48.
+// rhu(x0 * c + x1 * s, 30), not yet saturated; the sum stays below 2^48.
 __device__ __forceinline__ int turn(int x0, int c, int x1, int s) {
-  const long long t = (long long)x0 * c + (long long)x1 * s + (1ll << 29);
-  return sat16((int)(t >> 30));
+  const long long t = (long long)x0 * c + ((long long)x1 * s + (1ll << 29));
+  return (int)(t >> 30);
 }
 
 // VEC: an item is 16 dims of a head (8 pairs, or 16 dims past rotary_dim),
 // two 16-byte accesses.  Otherwise an item is one pair, or one dim past rotary_dim.
-template <bool VEC>
+template <bool VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
   extern __shared__ __align__(16) int32_t angles[];  // c [rows][half], then s
   int32_t* const sc = angles;
@@ -108,8 +106,8 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
     const int base = p.head * a.hd;
     if (p.slot < turning) {
       const int pair = VEC ? 8 * p.slot : p.slot;
-      i0 = base + (a.interleaved ? 2 * pair : pair);
-      i1 = a.interleaved ? i0 + (VEC ? 8 : 1) : i0 + a.half;
+      i0 = base + (INTERLEAVED ? 2 * pair : pair);
+      i1 = INTERLEAVED ? i0 + (VEC ? 8 : 1) : i0 + a.half;
       return pair;
     }
     i0 = base + 2 * a.half + (VEC ? 16 : 1) * (p.slot - turning);
@@ -178,37 +176,39 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
       if (VEC) {
         uint4 o0 = v0[k], o1 = v1[k];
         if (pair >= 0) {
-          int e0[8], e1[8], r0[8], r1[8], cw[8], sw[8];
+          int cw[8], sw[8], r0[8], r1[8];
 #pragma unroll
           for (int i = 0; i < 8; i += 4) {
             *reinterpret_cast<int4*>(cw + i) = *reinterpret_cast<const int4*>(c + i);
             *reinterpret_cast<int4*>(sw + i) = *reinterpret_cast<const int4*>(s + i);
           }
-          unpack8(v0[k], e0);
-          unpack8(v1[k], e1);
+          int e[16];
+          unpack8(v0[k], *reinterpret_cast<int(*)[8]>(e));
+          unpack8(v1[k], *reinterpret_cast<int(*)[8]>(e + 8));
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int x0 = a.interleaved ? (i < 4 ? e0[2 * i & 7] : e1[2 * i & 7]) : e0[i];
-            const int x1 = a.interleaved ? (i < 4 ? e0[(2 * i & 7) + 1] : e1[(2 * i & 7) + 1]) : e1[i];
+            const int x0 = e[INTERLEAVED ? 2 * i : i], x1 = e[INTERLEAVED ? 2 * i + 1 : 8 + i];
             r0[i] = turn(x0, cw[i], x1, -sw[i]);
             r1[i] = turn(x0, sw[i], x1, cw[i]);
           }
-          if (a.interleaved) {
-            const int m0[8] = {r0[0], r1[0], r0[1], r1[1], r0[2], r1[2], r0[3], r1[3]};
-            const int m1[8] = {r0[4], r1[4], r0[5], r1[5], r0[6], r1[6], r0[7], r1[7]};
-            o0 = pack8(m0);
-            o1 = pack8(m1);
+          if (INTERLEAVED) {
+            o0 = make_uint4(pack_sat16(r1[0], r0[0]), pack_sat16(r1[1], r0[1]), pack_sat16(r1[2], r0[2]),
+                            pack_sat16(r1[3], r0[3]));
+            o1 = make_uint4(pack_sat16(r1[4], r0[4]), pack_sat16(r1[5], r0[5]), pack_sat16(r1[6], r0[6]),
+                            pack_sat16(r1[7], r0[7]));
           } else {
-            o0 = pack8(r0);
-            o1 = pack8(r1);
+            o0 = make_uint4(pack_sat16(r0[1], r0[0]), pack_sat16(r0[3], r0[2]), pack_sat16(r0[5], r0[4]),
+                            pack_sat16(r0[7], r0[6]));
+            o1 = make_uint4(pack_sat16(r1[1], r1[0]), pack_sat16(r1[3], r1[2]), pack_sat16(r1[5], r1[4]),
+                            pack_sat16(r1[7], r1[6]));
           }
         }
         *reinterpret_cast<uint4*>(p + i0) = o0;
         *reinterpret_cast<uint4*>(p + i1) = o1;
       } else {
         const int x0 = (int)(int16_t)v0[k].x, x1 = (int)(int16_t)v1[k].x;
-        p[i0] = (int16_t)(pair >= 0 ? turn(x0, c[0], x1, -s[0]) : x0);
-        if (pair >= 0) p[i1] = (int16_t)turn(x0, s[0], x1, c[0]);
+        p[i0] = (int16_t)(pair >= 0 ? sat16(turn(x0, c[0], x1, -s[0])) : x0);
+        if (pair >= 0) p[i1] = (int16_t)sat16(turn(x0, s[0], x1, c[0]));
       }
     }
   }
@@ -232,7 +232,6 @@ cudaError_t launch_rotary(const int16_t* x, size_t rows, size_t heads, size_t hd
   a.heads = (int)heads;
   a.hd = (int)hd;
   a.half = (int)(rot.rotary_dim / 2);
-  a.interleaved = rot.interleaved != 0;
   a.backward = backward;
   a.amplitude = rot.amplitude;
   const bool vec = hd % 16 == 0 && a.half % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 &&
@@ -248,8 +247,9 @@ cudaError_t launch_rotary(const int16_t* x, size_t rows, size_t heads, size_t hd
   if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
   const double n = (double)rows * (double)heads * (double)hd;
   ProfScope prof("rotary", s, 3.0 * (double)rows * (double)heads * (double)rot.rotary_dim, 4.0 * n);
-  const cudaError_t e = launch_pdl(vec ? rotary_kernel<true> : rotary_kernel<false>, dim3((unsigned)blocks),
-                                   dim3(THREADS), 8 * r * (size_t)a.half, s, a);
+  auto* kernel = vec ? (rot.interleaved ? rotary_kernel<true, true> : rotary_kernel<true, false>)
+                     : (rot.interleaved ? rotary_kernel<false, true> : rotary_kernel<false, false>);
+  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)blocks), dim3(THREADS), 8 * r * (size_t)a.half, s, a);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
