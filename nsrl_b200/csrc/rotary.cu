@@ -6,12 +6,19 @@
 // of the circle and the remaining angle d (|d| <= 2^-11 turn = 0.0031 rad):
 // cos d = 1 - d^2 / 2 within 4e-12, sin d = d within 5e-9, both below 2^-27.
 //
-// Bound by memory: 2 bytes in and 2 out per element, against about 6 integer
-// instructions; the angle work is done once per (row, pair) into shared
-// memory and read by every head.  A block takes `rows` rows so that each of
-// its 256 threads has about four items (16 dims: two 16-byte loads and
-// stores) per head sweep, and asks for its first four items before it works
-// out the angles, which hides that work behind the loads.
+// Bound by memory (2 bytes in and 2 out per element) as long as integer
+// instructions are few: both integer pipes issue every other cycle.  So
+//  - the angles are worked out once per (row, pair) into shared memory and
+//    read by every head;
+//  - a Q30 factor is c = 2^15 ch + cl with |cl| <= 2^14, and
+//      rhu(x0 c - x1 s, 30) = (P + (Q >> 15)) >> 15,
+//      P = x0 ch - x1 sh,  Q = x0 cl - x1 sl + 2^29,
+//    exact in 32 bits (floor of a floor; |P| < 2^31 as c^2 + s^2 = 2^60,
+//    |Q| < 2^31): five multiply-adds and a shift, where the 64-bit sum of two
+//    widening products takes seven instructions.  An amplitude above 1 keeps
+//    the 64-bit form;
+//  - a thread keeps its column (head and pairs) and steps down the rows.
+// The loads of a thread's first rows are under way while it works out angles.
 #include <algorithm>
 
 #include "common.cuh"
@@ -22,9 +29,10 @@ namespace {
 
 __device__ const int32_t d_quarter_lut[257] = {NSRL_QUARTER_LUT_VALUES};
 
-constexpr int THREADS = 256;
-constexpr int MAX_PAIRS = 2048;  // (row, pair) angles of a block: 16 KB of shared memory
-constexpr int ITEMS = 4;         // items a thread loads ahead
+constexpr int MAX_THREADS = 256;
+constexpr int MAX_PAIRS = 1024;  // (row, pair) angles of a block: 16 KB of shared memory
+constexpr int AHEAD = 2;         // rows a thread loads ahead
+constexpr int ROWS = 4;          // rows a thread takes, where there are enough
 
 struct RotArgs {
   const int16_t* x;
@@ -36,6 +44,12 @@ struct RotArgs {
   int heads, hd, half, backward, amplitude;
   int block_rows;
 };
+
+__device__ __forceinline__ long long mad_wide(int x, int y, long long z) {
+  long long r;
+  asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(r) : "r"(x), "r"(y), "l"(z));
+  return r;
+}
 
 // Q30 cosine and sine of a 2^-64 turn (the integer recipe of nsrl_b200.h).
 __device__ __forceinline__ void cos_sin_q30(unsigned long long a, int amplitude, int& c, int& s) {
@@ -52,8 +66,8 @@ __device__ __forceinline__ void cos_sin_q30(unsigned long long a, int amplitude,
   const int r = __mulhi((int)(d >> 22), 1686629713);
   const int h256 = ((__mulhi(r, r) + (1 << 14)) >> 15) << 8;  // below 2^21
   const long long half = 1ll << 37;
-  c = C0 - (int)(((long long)C0 * h256 + (long long)S0 * r + half) >> 38);
-  s = S0 - (int)(((long long)S0 * h256 - (long long)C0 * r + half) >> 38);
+  c = C0 - (int)(mad_wide(C0, h256, mad_wide(S0, r, half)) >> 38);
+  s = S0 - (int)(mad_wide(S0, h256, mad_wide(C0, -r, half)) >> 38);
   if (amplitude != (1 << 30)) {
     // |c| may pass 2^30 by one, so an amplitude near 2 may reach 2^31: held to 2^31 - 1
     c = (int)max(-2147483647ll, min(2147483647ll, ((long long)c * amplitude + (1ll << 29)) >> 30));
@@ -61,154 +75,165 @@ __device__ __forceinline__ void cos_sin_q30(unsigned long long a, int amplitude,
   }
 }
 
-// rhu(x0 * c + x1 * s, 30), not yet saturated; the sum stays below 2^48.
-__device__ __forceinline__ int turn(int x0, int c, int x1, int s) {
-  const long long t = (long long)x0 * c + ((long long)x1 * s + (1ll << 29));
-  return (int)(t >> 30);
+// rhu(x0 * c + x1 * s, 30), not yet saturated.
+template <bool WIDE>
+__device__ __forceinline__ int turn(int x0, int ch, int cl, int x1, int sh, int sl) {
+  if (WIDE) return (int)(mad_wide(x0, ch, mad_wide(x1, sh, 1ll << 29)) >> 30);
+  const int p = x0 * ch + x1 * sh;
+  const int q = x0 * cl + (x1 * sl + (1 << 29));
+  int r;
+  asm("mad.hi.s32 %0, %1, %2, %3;" : "=r"(r) : "r"(q), "r"(1 << 17), "r"(p));  // p + (q >> 15)
+  return r >> 15;
 }
 
 // VEC: an item is 16 dims of a head (8 pairs, or 16 dims past rotary_dim),
 // two 16-byte accesses.  Otherwise an item is one pair, or one dim past rotary_dim.
-template <bool VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
-  extern __shared__ __align__(16) int32_t angles[];  // c [rows][half], then s
-  int32_t* const sc = angles;
-  int32_t* const ss = angles + a.block_rows * a.half;
+template <bool VEC, bool INTERLEAVED, bool WIDE>
+__global__ void __launch_bounds__(MAX_THREADS) rotary_kernel(const RotArgs a) {
+  extern __shared__ __align__(16) int32_t angles[];  // [4][rows][half]: ch, cl, sh, sl (WIDE: c, s in the first two)
+  const int angle_count = a.block_rows * a.half;
+  int32_t* const ch = angles;
+  int32_t* const cl = angles + angle_count;  // WIDE: s
+  int32_t* const sh = angles + 2 * angle_count;
+  int32_t* const sl = angles + 3 * angle_count;
   const long long row0 = (long long)blockIdx.x * a.block_rows;
   const int rows = (int)min((long long)a.block_rows, a.rows - row0);
   // items of a head: the pairs, then (out of place only) the dims that pass through
   const int turning = VEC ? a.half / 8 : a.half;
   const int passing = a.x == a.y ? 0 : (VEC ? (a.hd - 2 * a.half) / 16 : a.hd - 2 * a.half);
   const int per_head = turning + passing, per_row = per_head * a.heads;
-  const int items = rows * per_row;
+  const int down = max(1, (int)blockDim.x / per_row);  // rows the block takes at once
+  const int my_row = threadIdx.x / per_row;            // beyond `down`: this thread has no column
 
-  // An item's place, stepped from one to the next by THREADS in mixed radix:
-  // two divisions a thread instead of two an item.
-  struct Place {
-    int row, head, slot;
-  };
-  const int step_row = THREADS / per_row, step_head = THREADS % per_row / per_head, step_slot = THREADS % per_head;
-  auto next = [&](Place& p) {
-    p.slot += step_slot;
-    p.head += step_head;
-    p.row += step_row;
-    if (p.slot >= per_head) {
-      p.slot -= per_head;
-      ++p.head;
-    }
-    if (p.head >= a.heads) {
-      p.head -= a.heads;
-      ++p.row;
-    }
-  };
-  // element offsets of an item's two accesses within its row, and its first pair (-1: passes through)
-  auto offsets = [&](const Place& p, int& i0, int& i1) -> int {
-    const int base = p.head * a.hd;
-    if (p.slot < turning) {
-      const int pair = VEC ? 8 * p.slot : p.slot;
+  griddep_wait();
+  griddep_launch();
+  const int16_t* const x = a.x + row0 * a.ldx;
+  int16_t* const y = a.y + row0 * a.ldy;
+  // element offsets of a column's two accesses within a row, and its first pair (-1: passes through)
+  auto place = [&](int column, int& i0, int& i1) -> int {
+    const int head = column / per_head, slot = column - head * per_head, base = head * a.hd;
+    if (slot < turning) {
+      const int pair = VEC ? 8 * slot : slot;
       i0 = base + (INTERLEAVED ? 2 * pair : pair);
       i1 = INTERLEAVED ? i0 + (VEC ? 8 : 1) : i0 + a.half;
       return pair;
     }
-    i0 = base + 2 * a.half + (VEC ? 16 : 1) * (p.slot - turning);
+    i0 = base + 2 * a.half + (VEC ? 16 : 1) * (slot - turning);
     i1 = i0 + (VEC ? 8 : 0);
     return -1;
   };
-
-  griddep_wait();
-  griddep_launch();
-  uint4 v0[ITEMS], v1[ITEMS];
-  auto load = [&](const Place& p, uint4& u0, uint4& u1) {
-    int i0, i1;
-    offsets(p, i0, i1);
-    const int16_t* x = a.x + (row0 + p.row) * a.ldx;
+  auto load = [&](const int16_t* row, int i0, int i1, uint4& u0, uint4& u1) {
     if (VEC) {
-      u0 = *reinterpret_cast<const uint4*>(x + i0);
-      u1 = *reinterpret_cast<const uint4*>(x + i1);
+      u0 = *reinterpret_cast<const uint4*>(row + i0);
+      u1 = *reinterpret_cast<const uint4*>(row + i1);
     } else {
-      u0.x = (uint32_t)(uint16_t)x[i0];
-      u1.x = (uint32_t)(uint16_t)x[i1];
+      u0.x = (uint32_t)(uint16_t)row[i0];
+      u1.x = (uint32_t)(uint16_t)row[i1];
     }
   };
-  Place start;
-  start.row = threadIdx.x / per_row;
-  start.head = threadIdx.x % per_row / per_head;
-  start.slot = threadIdx.x % per_head;
-  Place at = start;
+
+  int column = my_row < down ? threadIdx.x - my_row * per_row : per_row;
+  int i0 = 0, i1 = 0, pair = -1;
+  uint4 v0[AHEAD], v1[AHEAD];
+  if (column < per_row) {
+    pair = place(column, i0, i1);
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    if (threadIdx.x + k * THREADS < items) load(at, v0[k], v1[k]);
-    next(at);
+    for (int k = 0; k < AHEAD; ++k)
+      if (my_row + k * down < rows) load(x + (my_row + k * down) * a.ldx, i0, i1, v0[k], v1[k]);
   }
   {
-    int row = threadIdx.x / a.half, pair = threadIdx.x % a.half;
-    const int down = THREADS / a.half, along = THREADS % a.half;
-    for (int i = threadIdx.x; i < rows * a.half; i += THREADS) {
+    int row = threadIdx.x / a.half, p = threadIdx.x - row * a.half;
+    const int step = blockDim.x / a.half, along = blockDim.x - step * a.half;
+    for (int i = threadIdx.x; i < rows * a.half; i += blockDim.x) {
       const long long r = row0 + row;
-      const long long p = a.positions ? (long long)a.positions[r] : (long long)((unsigned)r % a.seq_len);
+      const long long at = a.positions ? (long long)a.positions[r] : (long long)((unsigned)r % a.seq_len);
       int c, s;
-      cos_sin_q30((unsigned long long)p * a.turns[pair], a.amplitude, c, s);
-      sc[i] = c;
-      ss[i] = a.backward ? -s : s;
-      row += down;
-      pair += along;
-      if (pair >= a.half) {
-        pair -= a.half;
+      cos_sin_q30((unsigned long long)at * a.turns[p], a.amplitude, c, s);
+      if (a.backward) s = -s;
+      if (WIDE) {
+        ch[i] = c;
+        cl[i] = s;
+      } else {
+        const int h = (c + (1 << 14)) >> 15, g = (s + (1 << 14)) >> 15;
+        ch[i] = h;
+        cl[i] = c - (h << 15);
+        sh[i] = g;
+        sl[i] = s - (g << 15);
+      }
+      row += step;
+      p += along;
+      if (p >= a.half) {
+        p -= a.half;
         ++row;
       }
     }
   }
   __syncthreads();
 
-  at = start;
-  for (int it0 = threadIdx.x; it0 < items; it0 += ITEMS * THREADS) {
+  for (bool first = true; column < per_row; column += blockDim.x, first = false) {
+    if (!first) pair = place(column, i0, i1);
+    const int16_t* xr = x + my_row * a.ldx;
+    int16_t* yr = y + my_row * a.ldy;
+    int angle = my_row * a.half + pair;
+    for (int r = my_row; r < rows; r += AHEAD * down) {
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      const Place here = at;
-      next(at);
-      if (it0 + k * THREADS >= items) continue;
-      if (it0 >= ITEMS * THREADS) load(here, v0[k], v1[k]);  // past the items loaded ahead
-      int i0, i1;
-      const int pair = offsets(here, i0, i1);
-      int16_t* p = a.y + (row0 + here.row) * a.ldy;
-      const int32_t* c = sc + here.row * a.half + pair;
-      const int32_t* s = ss + here.row * a.half + pair;
-      if (VEC) {
-        uint4 o0 = v0[k], o1 = v1[k];
-        if (pair >= 0) {
-          int cw[8], sw[8], r0[8], r1[8];
+      for (int k = 0; k < AHEAD; ++k) {
+        if (r + k * down >= rows) break;
+        if (!first || r != my_row) load(xr, i0, i1, v0[k], v1[k]);  // past the rows loaded ahead
+        if (VEC) {
+          uint4 o0 = v0[k], o1 = v1[k];
+          if (pair >= 0) {
+            int e[16], t0[8], t1[8];
+            unpack8(v0[k], *reinterpret_cast<int(*)[8]>(e));
+            unpack8(v1[k], *reinterpret_cast<int(*)[8]>(e + 8));
 #pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            *reinterpret_cast<int4*>(cw + i) = *reinterpret_cast<const int4*>(c + i);
-            *reinterpret_cast<int4*>(sw + i) = *reinterpret_cast<const int4*>(s + i);
+            for (int q = 0; q < 8; q += 4) {
+              int f[4][4];
+#pragma unroll
+              for (int j = 0; j < (WIDE ? 2 : 4); ++j)
+                *reinterpret_cast<int4*>(f[j]) = *reinterpret_cast<const int4*>(angles + j * angle_count + angle + q);
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                const int i = q + m;
+                const int x0 = e[INTERLEAVED ? 2 * i : i], x1 = e[INTERLEAVED ? 2 * i + 1 : 8 + i];
+                if (WIDE) {
+                  t0[i] = turn<true>(x0, f[0][m], 0, x1, -f[1][m], 0);
+                  t1[i] = turn<true>(x0, f[1][m], 0, x1, f[0][m], 0);
+                } else {
+                  t0[i] = turn<false>(x0, f[0][m], f[1][m], x1, -f[2][m], -f[3][m]);
+                  t1[i] = turn<false>(x0, f[2][m], f[3][m], x1, f[0][m], f[1][m]);
+                }
+              }
+            }
+            if (INTERLEAVED) {
+              o0 = make_uint4(pack_sat16(t1[0], t0[0]), pack_sat16(t1[1], t0[1]), pack_sat16(t1[2], t0[2]),
+                              pack_sat16(t1[3], t0[3]));
+              o1 = make_uint4(pack_sat16(t1[4], t0[4]), pack_sat16(t1[5], t0[5]), pack_sat16(t1[6], t0[6]),
+                              pack_sat16(t1[7], t0[7]));
+            } else {
+              o0 = make_uint4(pack_sat16(t0[1], t0[0]), pack_sat16(t0[3], t0[2]), pack_sat16(t0[5], t0[4]),
+                              pack_sat16(t0[7], t0[6]));
+              o1 = make_uint4(pack_sat16(t1[1], t1[0]), pack_sat16(t1[3], t1[2]), pack_sat16(t1[5], t1[4]),
+                              pack_sat16(t1[7], t1[6]));
+            }
           }
-          int e[16];
-          unpack8(v0[k], *reinterpret_cast<int(*)[8]>(e));
-          unpack8(v1[k], *reinterpret_cast<int(*)[8]>(e + 8));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int x0 = e[INTERLEAVED ? 2 * i : i], x1 = e[INTERLEAVED ? 2 * i + 1 : 8 + i];
-            r0[i] = turn(x0, cw[i], x1, -sw[i]);
-            r1[i] = turn(x0, sw[i], x1, cw[i]);
-          }
-          if (INTERLEAVED) {
-            o0 = make_uint4(pack_sat16(r1[0], r0[0]), pack_sat16(r1[1], r0[1]), pack_sat16(r1[2], r0[2]),
-                            pack_sat16(r1[3], r0[3]));
-            o1 = make_uint4(pack_sat16(r1[4], r0[4]), pack_sat16(r1[5], r0[5]), pack_sat16(r1[6], r0[6]),
-                            pack_sat16(r1[7], r0[7]));
+          *reinterpret_cast<uint4*>(yr + i0) = o0;
+          *reinterpret_cast<uint4*>(yr + i1) = o1;
+        } else {
+          const int x0 = (int)(int16_t)v0[k].x, x1 = (int)(int16_t)v1[k].x;
+          if (pair < 0) {
+            yr[i0] = (int16_t)x0;
+          } else if (WIDE) {
+            yr[i0] = (int16_t)sat16(turn<true>(x0, ch[angle], 0, x1, -cl[angle], 0));
+            yr[i1] = (int16_t)sat16(turn<true>(x0, cl[angle], 0, x1, ch[angle], 0));
           } else {
-            o0 = make_uint4(pack_sat16(r0[1], r0[0]), pack_sat16(r0[3], r0[2]), pack_sat16(r0[5], r0[4]),
-                            pack_sat16(r0[7], r0[6]));
-            o1 = make_uint4(pack_sat16(r1[1], r1[0]), pack_sat16(r1[3], r1[2]), pack_sat16(r1[5], r1[4]),
-                            pack_sat16(r1[7], r1[6]));
+            yr[i0] = (int16_t)sat16(turn<false>(x0, ch[angle], cl[angle], x1, -sh[angle], -sl[angle]));
+            yr[i1] = (int16_t)sat16(turn<false>(x0, sh[angle], sl[angle], x1, ch[angle], cl[angle]));
           }
         }
-        *reinterpret_cast<uint4*>(p + i0) = o0;
-        *reinterpret_cast<uint4*>(p + i1) = o1;
-      } else {
-        const int x0 = (int)(int16_t)v0[k].x, x1 = (int)(int16_t)v1[k].x;
-        p[i0] = (int16_t)(pair >= 0 ? sat16(turn(x0, c[0], x1, -s[0])) : x0);
-        if (pair >= 0) p[i1] = (int16_t)sat16(turn(x0, s[0], x1, c[0]));
+        xr += down * a.ldx;
+        yr += down * a.ldy;
+        angle += down * a.half;
       }
     }
   }
@@ -236,20 +261,27 @@ cudaError_t launch_rotary(const int16_t* x, size_t rows, size_t heads, size_t hd
   a.amplitude = rot.amplitude;
   const bool vec = hd % 16 == 0 && a.half % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 &&
                    ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
-  // Rows of a block: about ITEMS items a thread, at least one block an SM
-  // while there are rows for it, and angles that fit the shared memory.
-  const size_t per_row = std::max<size_t>(1, heads * (vec ? hd / 16 : hd - (size_t)a.half));
-  size_t r = std::max<size_t>(1, (size_t)(ITEMS * THREADS) / per_row);
+  const bool wide = rot.amplitude > (1 << 30);
+  // A block is a whole number of rows wide where a row has at most MAX_THREADS
+  // items.  It takes ROWS times that many rows, but leaves every SM a block
+  // while there are rows for it, and keeps to its angles' shared memory.
+  const size_t passing = x == y ? 0 : hd - rot.rotary_dim;
+  const size_t per_row = heads * (vec ? (rot.rotary_dim + passing) / 16 : (size_t)a.half + passing);
+  const size_t down = std::max<size_t>(1, MAX_THREADS / per_row);
+  size_t r = ROWS * down;
   r = std::min(r, std::max<size_t>(1, rows / 148));
   r = std::min(r, std::max<size_t>(1, (size_t)MAX_PAIRS / (size_t)a.half));
   a.block_rows = (int)r;
+  const size_t threads = (std::min<size_t>(MAX_THREADS, std::min(down, r) * per_row) + 31) / 32 * 32;
   const size_t blocks = (rows + r - 1) / r;
   if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
   const double n = (double)rows * (double)heads * (double)hd;
   ProfScope prof("rotary", s, 3.0 * (double)rows * (double)heads * (double)rot.rotary_dim, 4.0 * n);
-  auto* kernel = vec ? (rot.interleaved ? rotary_kernel<true, true> : rotary_kernel<true, false>)
-                     : (rot.interleaved ? rotary_kernel<false, true> : rotary_kernel<false, false>);
-  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)blocks), dim3(THREADS), 8 * r * (size_t)a.half, s, a);
+  auto* kernel = vec ? (rot.interleaved ? (wide ? rotary_kernel<true, true, true> : rotary_kernel<true, true, false>)
+                                        : (wide ? rotary_kernel<true, false, true> : rotary_kernel<true, false, false>))
+                     : (rot.interleaved ? (wide ? rotary_kernel<false, true, true> : rotary_kernel<false, true, false>)
+                                        : (wide ? rotary_kernel<false, false, true> : rotary_kernel<false, false, false>));
+  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 16 * r * (size_t)a.half, s, a);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
