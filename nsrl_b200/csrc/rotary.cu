@@ -42,8 +42,15 @@ struct RotArgs {
   const int32_t* positions;
   unsigned seq_len;
   int heads, hd, half, backward, amplitude;
-  int block_rows;
+  int block_rows;         // rows of a block
+  int turning, per_head;  // items of a head that turn, and all of them (out of place: dims that pass through too)
+  int per_row, down;      // items of a row; rows the block takes at once
+  int step, along;        // blockDim.x = step * half + along
+  unsigned by_row, by_head, by_half;  // ceil(2^22 / d) of the three divisors
 };
+
+// n / d for n < 1024 by m = ceil(2^22 / d): exact while n d < 2^22, and 0 for larger d.
+__device__ __forceinline__ int small_div(unsigned n, unsigned m) { return (int)((n * m) >> 22); }
 
 __device__ __forceinline__ long long mad_wide(int x, int y, long long z) {
   long long r;
@@ -75,12 +82,12 @@ __device__ __forceinline__ void cos_sin_q30(unsigned long long a, int amplitude,
   }
 }
 
-// rhu(x0 * c + x1 * s, 30), not yet saturated.
-template <bool WIDE>
+// rhu(x0 * c - x1 * s, 30) (MINUS) or rhu(x0 * c + x1 * s, 30), not yet saturated.
+template <bool WIDE, bool MINUS>
 __device__ __forceinline__ int turn(int x0, int ch, int cl, int x1, int sh, int sl) {
-  if (WIDE) return (int)(mad_wide(x0, ch, mad_wide(x1, sh, 1ll << 29)) >> 30);
-  const int p = x0 * ch + x1 * sh;
-  const int q = x0 * cl + (x1 * sl + (1 << 29));
+  if (WIDE) return (int)(mad_wide(x0, ch, mad_wide(MINUS ? -x1 : x1, sh, 1ll << 29)) >> 30);
+  const int p = MINUS ? x0 * ch - x1 * sh : x0 * ch + x1 * sh;
+  const int q = MINUS ? (x0 * cl + (1 << 29)) - x1 * sl : (x0 * cl + (1 << 29)) + x1 * sl;
   int r;
   asm("mad.hi.s32 %0, %1, %2, %3;" : "=r"(r) : "r"(q), "r"(1 << 17), "r"(p));  // p + (q >> 15)
   return r >> 15;
@@ -98,20 +105,16 @@ __global__ void __launch_bounds__(MAX_THREADS) rotary_kernel(const RotArgs a) {
   int32_t* const sl = angles + 3 * angle_count;
   const long long row0 = (long long)blockIdx.x * a.block_rows;
   const int rows = (int)min((long long)a.block_rows, a.rows - row0);
-  // items of a head: the pairs, then (out of place only) the dims that pass through
-  const int turning = VEC ? a.half / 8 : a.half;
-  const int passing = a.x == a.y ? 0 : (VEC ? (a.hd - 2 * a.half) / 16 : a.hd - 2 * a.half);
-  const int per_head = turning + passing, per_row = per_head * a.heads;
-  const int down = max(1, (int)blockDim.x / per_row);  // rows the block takes at once
-  const int my_row = threadIdx.x / per_row;            // beyond `down`: this thread has no column
+  const int turning = a.turning, per_head = a.per_head, per_row = a.per_row, down = a.down;
+  const int my_row = small_div(threadIdx.x, a.by_row);  // beyond `down`: this thread has no column
 
   griddep_wait();
   griddep_launch();
   const int16_t* const x = a.x + row0 * a.ldx;
   int16_t* const y = a.y + row0 * a.ldy;
   // element offsets of a column's two accesses within a row, and its first pair (-1: passes through)
-  auto place = [&](int column, int& i0, int& i1) -> int {
-    const int head = column / per_head, slot = column - head * per_head, base = head * a.hd;
+  auto place = [&](int column, int head, int& i0, int& i1) -> int {
+    const int slot = column - head * per_head, base = head * a.hd;
     if (slot < turning) {
       const int pair = VEC ? 8 * slot : slot;
       i0 = base + (INTERLEAVED ? 2 * pair : pair);
@@ -136,14 +139,13 @@ __global__ void __launch_bounds__(MAX_THREADS) rotary_kernel(const RotArgs a) {
   int i0 = 0, i1 = 0, pair = -1;
   uint4 v0[AHEAD], v1[AHEAD];
   if (column < per_row) {
-    pair = place(column, i0, i1);
+    pair = place(column, small_div(column, a.by_head), i0, i1);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
       if (my_row + k * down < rows) load(x + (my_row + k * down) * a.ldx, i0, i1, v0[k], v1[k]);
   }
   {
-    int row = threadIdx.x / a.half, p = threadIdx.x - row * a.half;
-    const int step = blockDim.x / a.half, along = blockDim.x - step * a.half;
+    int row = small_div(threadIdx.x, a.by_half), p = threadIdx.x - row * a.half;
     for (int i = threadIdx.x; i < rows * a.half; i += blockDim.x) {
       const long long r = row0 + row;
       const long long at = a.positions ? (long long)a.positions[r] : (long long)((unsigned)r % a.seq_len);
@@ -160,8 +162,8 @@ __global__ void __launch_bounds__(MAX_THREADS) rotary_kernel(const RotArgs a) {
         sh[i] = g;
         sl[i] = s - (g << 15);
       }
-      row += step;
-      p += along;
+      row += a.step;
+      p += a.along;
       if (p >= a.half) {
         p -= a.half;
         ++row;
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(MAX_THREADS) rotary_kernel(const RotArgs a) {
   __syncthreads();
 
   for (bool first = true; column < per_row; column += blockDim.x, first = false) {
-    if (!first) pair = place(column, i0, i1);
+    if (!first) pair = place(column, column / per_head, i0, i1);
     const int16_t* xr = x + my_row * a.ldx;
     int16_t* yr = y + my_row * a.ldy;
     int angle = my_row * a.half + pair;
@@ -197,11 +199,11 @@ __global__ void __launch_bounds__(MAX_THREADS) rotary_kernel(const RotArgs a) {
                 const int i = q + m;
                 const int x0 = e[INTERLEAVED ? 2 * i : i], x1 = e[INTERLEAVED ? 2 * i + 1 : 8 + i];
                 if (WIDE) {
-                  t0[i] = turn<true>(x0, f[0][m], 0, x1, -f[1][m], 0);
-                  t1[i] = turn<true>(x0, f[1][m], 0, x1, f[0][m], 0);
+                  t0[i] = turn<true, true>(x0, f[0][m], 0, x1, f[1][m], 0);
+                  t1[i] = turn<true, false>(x0, f[1][m], 0, x1, f[0][m], 0);
                 } else {
-                  t0[i] = turn<false>(x0, f[0][m], f[1][m], x1, -f[2][m], -f[3][m]);
-                  t1[i] = turn<false>(x0, f[2][m], f[3][m], x1, f[0][m], f[1][m]);
+                  t0[i] = turn<false, true>(x0, f[0][m], f[1][m], x1, f[2][m], f[3][m]);
+                  t1[i] = turn<false, false>(x0, f[2][m], f[3][m], x1, f[0][m], f[1][m]);
                 }
               }
             }
@@ -224,11 +226,11 @@ __global__ void __launch_bounds__(MAX_THREADS) rotary_kernel(const RotArgs a) {
           if (pair < 0) {
             yr[i0] = (int16_t)x0;
           } else if (WIDE) {
-            yr[i0] = (int16_t)sat16(turn<true>(x0, ch[angle], 0, x1, -cl[angle], 0));
-            yr[i1] = (int16_t)sat16(turn<true>(x0, cl[angle], 0, x1, ch[angle], 0));
+            yr[i0] = (int16_t)sat16(turn<true, true>(x0, ch[angle], 0, x1, cl[angle], 0));
+            yr[i1] = (int16_t)sat16(turn<true, false>(x0, cl[angle], 0, x1, ch[angle], 0));
           } else {
-            yr[i0] = (int16_t)sat16(turn<false>(x0, ch[angle], cl[angle], x1, -sh[angle], -sl[angle]));
-            yr[i1] = (int16_t)sat16(turn<false>(x0, sh[angle], sl[angle], x1, ch[angle], cl[angle]));
+            yr[i0] = (int16_t)sat16(turn<false, true>(x0, ch[angle], cl[angle], x1, sh[angle], sl[angle]));
+            yr[i1] = (int16_t)sat16(turn<false, false>(x0, sh[angle], sl[angle], x1, ch[angle], cl[angle]));
           }
         }
         xr += down * a.ldx;
@@ -265,14 +267,24 @@ cudaError_t launch_rotary(const int16_t* x, size_t rows, size_t heads, size_t hd
   // A block is a whole number of rows wide where a row has at most MAX_THREADS
   // items.  It takes ROWS times that many rows, but leaves every SM a block
   // while there are rows for it, and keeps to its angles' shared memory.
-  const size_t passing = x == y ? 0 : hd - rot.rotary_dim;
-  const size_t per_row = heads * (vec ? (rot.rotary_dim + passing) / 16 : (size_t)a.half + passing);
-  const size_t down = std::max<size_t>(1, MAX_THREADS / per_row);
-  size_t r = ROWS * down;
-  r = std::min(r, std::max<size_t>(1, rows / 148));
+  const int unit = vec ? 8 : 1;
+  a.turning = a.half / unit;
+  a.per_head = a.turning + (x == y ? 0 : ((int)hd - 2 * a.half) / (vec ? 16 : 1));
+  a.per_row = a.per_head * a.heads;
+  size_t r = std::max<size_t>(1, MAX_THREADS / (size_t)a.per_row);
+  size_t wide_rows = r;
+  r = std::min(ROWS * r, std::max<size_t>(1, rows / 148));
   r = std::min(r, std::max<size_t>(1, (size_t)MAX_PAIRS / (size_t)a.half));
+  wide_rows = std::min(wide_rows, r);
   a.block_rows = (int)r;
-  const size_t threads = (std::min<size_t>(MAX_THREADS, std::min(down, r) * per_row) + 31) / 32 * 32;
+  a.down = (int)wide_rows;
+  const size_t threads = (std::min<size_t>(MAX_THREADS, wide_rows * (size_t)a.per_row) + 31) / 32 * 32;
+  a.step = (int)threads / a.half;
+  a.along = (int)threads % a.half;
+  auto magic = [](int d) { return ((1u << 22) + (unsigned)d - 1) / (unsigned)d; };
+  a.by_row = magic(a.per_row);
+  a.by_head = magic(a.per_head);
+  a.by_half = magic(a.half);
   const size_t blocks = (rows + r - 1) / r;
   if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
   const double n = (double)rows * (double)heads * (double)hd;
