@@ -48,21 +48,6 @@ def _lib():
     return L
 
 
-def _array(t: torch.Tensor, dtype, shape, what: str) -> int:
-    """The address of a contiguous tensor on the current device, of this type and shape."""
-    core._on_current_device(t, dtype, what)
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        raise core.NsrlError(f"{what} must be contiguous and of shape {shape}")
-    return t.data_ptr()
-
-
-def _rows(t: torch.Tensor, rows: int, cols: int, what: str) -> tuple[int, int]:
-    core._on_current_device(t, torch.int16, what)
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
-        raise core.NsrlError(f"{what} must be [{rows}, {cols}] with contiguous columns")
-    return t.data_ptr(), core._row_stride(t)
-
-
 class Q4Cache:
     """Codes and scales of `capacity` slots for every (sequence, head), empty at the start.
 
@@ -95,57 +80,66 @@ class Q4Cache:
         groups = max(1, self.head_dim // GROUP)
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.scores, self.positions = scores, positions
-        self.device = k_codes.device
-        ptr = [_array(k_codes, torch.uint8, (B, H, cap, half), "k_codes"),
-               _array(v_codes, torch.uint8, (B, H, cap, half), "v_codes"),
-               _array(k_scales, torch.int32, (B, H, cap, groups), "k_scales"),
-               _array(v_scales, torch.int32, (B, H, cap, groups), "v_scales"),
-               None if scores is None else _array(scores, torch.int32, (B, H, cap), "scores"),
-               None if positions is None else _array(positions, torch.int32, (B, H, cap), "positions")]
+        dev = torch.cuda.current_device()
+        ptr = [core._array(k_codes, torch.uint8, (B, H, cap, half), dev, "k_codes"),
+               core._array(v_codes, torch.uint8, (B, H, cap, half), dev, "v_codes"),
+               core._array(k_scales, torch.int32, (B, H, cap, groups), dev, "k_scales"),
+               core._array(v_scales, torch.int32, (B, H, cap, groups), dev, "v_scales"),
+               None if scores is None else core._array(scores, torch.int32, (B, H, cap), dev, "scores"),
+               None if positions is None else core._array(positions, torch.int32, (B, H, cap), dev, "positions")]
+        self.device, self._dev = k_codes.device, dev
+        self._cols = H * self.head_dim
         self._c = Q4CacheC(*ptr, B, H, self.head_dim, cap)
         self._ref = C.byref(self._c)
 
     def c(self) -> Q4CacheC:
         return self._c
 
-    def _per_sequence(self, t: Optional[torch.Tensor], what: str) -> Optional[int]:
-        return None if t is None else _array(t, torch.int32, (self.batch,), what)
+    def _per_sequence(self, t: torch.Tensor, what: str) -> int:
+        return core._array(t, torch.int32, (self.batch,), self._dev, what)
+
+    def _stream(self) -> int:
+        if torch.cuda.current_device() != self._dev:
+            raise core.NsrlError(f"the cache is on {self.device}, not on the current device")
+        return core._raw_stream(self._dev)
 
     # ---- enqueue only
     def launch_append(self, k, v, starts, counts=None, positions=None, status: core.Status = None) -> int:
         """k, v: int16 [batch * tokens, heads * head_dim] of one row stride (nsrl_q4_cache_append)."""
-        rows = k.shape[0]
-        if rows % max(1, self.batch):
-            raise core.NsrlError("k must hold the same number of rows for every sequence")
-        cols = self.heads * self.head_dim
-        kp, ld = _rows(k, rows, cols, "k")
-        vp, ldv = _rows(v, rows, cols, "v")
-        if rows > 1 and ld != ldv:
+        rows, cols = k.shape[0], self._cols
+        if rows % max(1, self.batch) or k.shape[1] != cols or v.shape[1] != cols:
+            raise core.NsrlError("k and v must be [batch * tokens, heads * head_dim]")
+        stream = self._stream()
+        kp, vp = core._rows(k, rows, cols, self._dev, "k"), core._rows(v, rows, cols, self._dev, "v")
+        ld = core._row_stride(k)
+        if rows > 1 and v.stride(0) != ld:
             raise core.NsrlError("k and v must have one row stride")
-        self._here()
         return _lib().nsrl_q4_cache_append(self._ref, kp, vp, ld, rows // max(1, self.batch),
-                                           self._per_sequence(starts, "starts"), self._per_sequence(counts, "counts"),
-                                           self._per_sequence(positions, "positions"), status.buf.data_ptr(),
-                                           core._stream())
+                                           self._per_sequence(starts, "starts"),
+                                           None if counts is None else self._per_sequence(counts, "counts"),
+                                           None if positions is None else self._per_sequence(positions, "positions"),
+                                           status.buf.data_ptr(), stream)
 
     def launch_read(self, starts, k, v, status: core.Status) -> int:
         """k, v: int16 [batch, heads, tokens, head_dim], written (nsrl_q4_cache_read)."""
         if k.dim() != 4:
             raise core.NsrlError("k must be [batch, heads, tokens, head_dim]")
-        shape = (self.batch, self.heads, k.shape[2], self.head_dim)
-        kp, vp = _array(k, torch.int16, shape, "k"), _array(v, torch.int16, shape, "v")
-        self._here()
-        return _lib().nsrl_q4_cache_read(self._ref, self._per_sequence(starts, "starts"), k.shape[2], kp, vp,
-                                         status.buf.data_ptr(), core._stream())
+        stream, tokens = self._stream(), k.shape[2]
+        shape = (self.batch, self.heads, tokens, self.head_dim)
+        return _lib().nsrl_q4_cache_read(self._ref, None if starts is None else self._per_sequence(starts, "starts"),
+                                         tokens, core._array(k, torch.int16, shape, self._dev, "k"),
+                                         core._array(v, torch.int16, shape, self._dev, "v"), status.buf.data_ptr(),
+                                         stream)
 
     def launch_attend(self, q, lens, ctx, status: core.Status) -> int:
         """q: int16 [batch, heads * head_dim] rows, ctx likewise and contiguous (nsrl_attention_decode_q4)."""
-        cols = self.heads * self.head_dim
-        qp, ldq = _rows(q, self.batch, cols, "q")
-        cp = _array(ctx, torch.int16, (self.batch, cols), "ctx")
-        self._here()
-        return _lib().nsrl_attention_decode_q4(qp, ldq, self._ref, self._per_sequence(lens, "lens"), cp,
-                                               status.buf.data_ptr(), core._stream())
+        stream, cols = self._stream(), self._cols
+        qp = core._rows(q, self.batch, cols, self._dev, "q")
+        if q.shape[1] != cols:
+            raise core.NsrlError("q must be [batch, heads * head_dim]")
+        return _lib().nsrl_attention_decode_q4(qp, core._row_stride(q), self._ref, self._per_sequence(lens, "lens"),
+                                               core._array(ctx, torch.int16, (self.batch, cols), self._dev, "ctx"),
+                                               status.buf.data_ptr(), stream)
 
     def evict_workspace_bytes(self, keep: int) -> int:
         return _lib().nsrl_q4_cache_evict_workspace_size(self._ref, keep)
@@ -153,18 +147,13 @@ class Q4Cache:
     def launch_evict(self, lens, next_positions, keep, sinks, recent, scores_out, positions_out, lens_out, ws,
                      status: core.Status) -> int:
         """nsrl_q4_cache_evict; the outputs may be lens and the cache's own scores and positions."""
-        shape = (self.batch, self.heads, self.capacity)
-        core._on_current_device(ws, torch.uint8, "the workspace")
-        self._here()
+        stream, shape = self._stream(), (self.batch, self.heads, self.capacity)
         return _lib().nsrl_q4_cache_evict(
             self._ref, self._per_sequence(lens, "lens"), self._per_sequence(next_positions, "next_positions"), keep,
-            sinks, recent, _array(scores_out, torch.int32, shape, "scores_out"),
-            _array(positions_out, torch.int32, shape, "positions_out"), self._per_sequence(lens_out, "lens_out"),
-            ws.data_ptr(), ws.numel(), status.buf.data_ptr(), core._stream())
-
-    def _here(self):
-        if self.device.index != torch.cuda.current_device():
-            raise core.NsrlError(f"the cache is on {self.device}, not on the current device")
+            sinks, recent, core._array(scores_out, torch.int32, shape, self._dev, "scores_out"),
+            core._array(positions_out, torch.int32, shape, self._dev, "positions_out"),
+            self._per_sequence(lens_out, "lens_out"), core._array(ws, torch.uint8, ws.shape, self._dev, "the workspace"),
+            ws.numel(), status.buf.data_ptr(), stream)
 
     # ---- checked calls
     def append(self, k, v, starts, counts=None, positions=None) -> Optional[bool]:
@@ -211,15 +200,16 @@ def prenorm_attention_decode_block_q4(x, rms_gamma, rms_eps, q, k, v, o, cache: 
     B, d = x.shape
     if B != cache.batch or g.numel() != d:
         raise core.NsrlError("x must be [cache.batch, d] and rms_gamma [d]")
-    core._on_current_device(x, torch.int16, "x")
-    cache._here()
+    stream = cache._stream()
+    xp = core._rows(x, B, d, cache._dev, "x")
+    lp = cache._per_sequence(lens, "lens")
+    pp = None if positions is None else cache._per_sequence(positions, "positions")
     y = torch.empty_like(x)
     ws = core.workspace(L.nsrl_decode_block_q4_workspace_size(B, d, cache.heads))
     st = core.Status()
     ps = [l.c() for l in (q, k, v, o)]
     h = core._run(lambda: L.nsrl_prenorm_attention_decode_block_q4(
-        x.data_ptr(), B, d, cache.heads, g.data_ptr(), rms_eps, *[C.byref(p) for p in ps],
-        None if rotary is None else C.byref(rotary.c()), cache._ref, cache._per_sequence(lens, "lens"),
-        cache._per_sequence(positions, "positions"), y.data_ptr(), ws.data_ptr(), ws.numel(), st.buf.data_ptr(),
-        core._stream()), st)
+        xp, B, d, cache.heads, g.data_ptr(), rms_eps, *[C.byref(p) for p in ps],
+        None if rotary is None else C.byref(rotary.c()), cache._ref, lp, pp, y.data_ptr(), ws.data_ptr(), ws.numel(),
+        st.buf.data_ptr(), stream), st)
     return None if h is None else (y, h.attention_saturations)

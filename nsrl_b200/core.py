@@ -171,12 +171,36 @@ def _i16(x: torch.Tensor) -> torch.Tensor:
     return x.contiguous()
 
 
-def _on_current_device(t: torch.Tensor, dtype, what: str):
-    """Raises unless t is a tensor of this type on the current CUDA device (the calls run on its stream)."""
+def _raw_stream(device: int) -> int:
+    """The current stream of a device as an address (torch.cuda.current_stream() takes 3 us to say it)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _refuse(t, dtype, device: int, what: str, shape: str):
+    """Says what is wrong with a tensor that a launch does not take."""
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
         raise NsrlError(f"{what} must be a CUDA tensor of {dtype}")
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != device:
         raise NsrlError(f"{what} is on {t.device}, not on the current device")
+    raise NsrlError(f"{what} must be {shape}")
+
+
+def _array(t: torch.Tensor, dtype, shape, device: int, what: str) -> int:
+    """The address of a contiguous tensor on the current device, of this type and shape."""
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != device or t.shape != shape
+            or not t.is_contiguous()):
+        _refuse(t, dtype, device, what, f"contiguous and of shape {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, rows: int, cols: int, device: int, what: str) -> int:
+    """The address of int16 rows of at least `cols` contiguous columns on the current device."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int16 or t.get_device() != device or t.dim() != 2:
+        _refuse(t, torch.int16, device, what, "rows")
+    n, width = t.shape
+    if n != rows or width < cols or (width > 1 and t.stride(1) != 1):
+        _refuse(t, torch.int16, device, what, f"{rows} rows of at least {cols} contiguous columns")
+    return t.data_ptr()
 
 
 def _row_stride(t: torch.Tensor) -> int:

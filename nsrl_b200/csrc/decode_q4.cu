@@ -558,7 +558,9 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
 template <int HD>
 cudaError_t launch_attend(const AttendArgs& a, int parts, size_t share, cudaStream_t s) {
   const size_t smem = Q4Shape<HD>::STAGES * Q4Shape<HD>::STAGE_BYTES + share * sizeof(int32_t);
-  cudaError_t e = cudaFuncSetAttribute(attend_q4_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  constexpr int MOST = Q4Shape<HD>::STAGES * Q4Shape<HD>::STAGE_BYTES + (int)MAX_SHARE * 4;
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_smem((const void*)attend_q4_kernel<HD>, MOST, done);
   if (e == cudaSuccess && parts > 8)
     e = cudaFuncSetAttribute(attend_q4_kernel<HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;

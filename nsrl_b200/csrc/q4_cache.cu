@@ -529,9 +529,8 @@ cudaError_t launch_q4_evict(const nsrl_q4_cache& c, const int32_t* lens, const i
                    : threads == 512 ? q4_select_kernel<512, 16>
                                     : q4_select_kernel<1024, 16>;
     ProfScope prof("q4_select", s, 0.0, 8.0 * (double)bh * (double)c.capacity);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess)
-      e = launch_pdl(kernel, dim3((unsigned)bh), dim3(threads), smem, s, a);
+    // the bitmap of the largest capacity is 32 KB: within the default limit
+    const cudaError_t e = launch_pdl(kernel, dim3((unsigned)bh), dim3(threads), smem, s, a);
     if (e != cudaSuccess) return e;
   }
   // moves of a CTA's step: 128 (32 at 256 dims), as many CTAs a row as its moves may need, 64 at most

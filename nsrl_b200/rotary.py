@@ -97,6 +97,7 @@ class Rotary:
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64,
                                   device=core._dev())
         self._c = RotaryC(self.turns.data_ptr(), rotary_dim, LAYOUTS[layout], q30)
+        self._ref = C.byref(self._c)
 
     def c(self) -> RotaryC:
         return self._c
@@ -108,28 +109,22 @@ class Rotary:
         positions: int32 [rows], or None for row % seq_len.  out may be x (in
         place); by default a new [rows, heads * head_dim] tensor.  Enqueues on
         the current stream without waiting; None on an invalid shape."""
-        L = _lib()
-        core._on_current_device(x, torch.int16, "x")
+        L, dev = _lib(), torch.cuda.current_device()
         cols = heads * self.head_dim
-        if x.dim() != 2 or x.shape[1] < cols or (x.shape[1] > 1 and x.stride(1) != 1):
-            raise core.NsrlError("x must be rows of at least heads * head_dim contiguous columns")
         rows = x.shape[0]
-        if positions is not None:
-            core._on_current_device(positions, torch.int32, "positions")
-            if positions.numel() != rows or not positions.is_contiguous():
-                raise core.NsrlError("positions must be contiguous, one per row")
-        core._on_current_device(self.turns, torch.int64, "the rotary turns")
-        y = torch.empty((rows, cols), dtype=torch.int16, device=x.device) if out is None else out
-        if out is not None:
-            core._on_current_device(y, torch.int16, "out")
-            if y.dim() != 2 or y.shape[0] != rows or y.shape[1] < cols or (y.shape[1] > 1 and y.stride(1) != 1):
-                raise core.NsrlError("out must be rows like x's")
+        xp = core._rows(x, rows, cols, dev, "x")
+        pp = None if positions is None else core._array(positions, torch.int32, (rows,), dev, "positions")
+        if self.turns.get_device() != dev:
+            core._refuse(self.turns, torch.int64, dev, "the rotary plan", "on the current device")
+        if out is None:
+            out = torch.empty((rows, cols), dtype=torch.int16, device=x.device)
+        yp = core._rows(out, rows, cols, dev, "out")
         if rows == 0:
-            return y
-        r = L.nsrl_rotary_rows(x.data_ptr(), rows, heads, self.head_dim, core._row_stride(x), C.byref(self._c),
-                               None if positions is None else positions.data_ptr(), seq_len, int(backward),
-                               y.data_ptr(), core._row_stride(y), core._stream())
+            return out
+        r = L.nsrl_rotary_rows(xp, rows, heads, self.head_dim, core._row_stride(x), self._ref, pp, seq_len,
+                               1 if backward else 0, yp, core._row_stride(out), core._raw_stream(dev))
+        if r == core.NSRL_OK:
+            return out
         if r == core.NSRL_INVALID_SHAPE:
             return None
         core._check(r)
-        return y
