@@ -286,10 +286,15 @@ nsrl_status nsrl_q4_cache_read(const nsrl_q4_cache* cache, const int32_t* starts
  * in place of int16 ones; the same logits, base-2 softmax and rounding, so on
  * equal values the same context.  ctx: [batch][heads * head_dim].  With
  * cache->scores, the Q15 weight of each slot is added to its score
- * (saturating at 2^31 - 1).  Capacity at most nsrl_q4_cache_max_capacity(). */
+ * (saturating at 2^31 - 1).  Capacity at most nsrl_q4_cache_max_capacity().
+ * workspace: nsrl_attention_decode_q4_workspace_size(cache) bytes (0 for a
+ * small cache: NULL is fine then), 256-byte aligned, its contents of no
+ * account before and after. */
 size_t nsrl_q4_cache_max_capacity(void);
+size_t nsrl_attention_decode_q4_workspace_size(const nsrl_q4_cache* cache);
 nsrl_status nsrl_attention_decode_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache* cache, const int32_t* lens,
-                                     int16_t* ctx, nsrl_device_status* status, void* stream);
+                                     int16_t* ctx, void* workspace, size_t workspace_bytes,
+                                     nsrl_device_status* status, void* stream);
 
 /* Cuts every (sequence, head) of more than `keep` slots to `keep`.  Slots
  * whose position is below `sinks`, or at least next_positions[b] - recent
@@ -315,7 +320,7 @@ nsrl_status nsrl_q4_cache_evict(const nsrl_q4_cache* cache, const int32_t* lens,
  * lens[b]), its k and v enter slot lens[b] (device int32, 0..capacity - 1),
  * and its query attends over slots 0 .. lens[b].  The caller advances lens
  * (and positions) after every layer of the step, and evicts between steps. */
-size_t nsrl_decode_block_q4_workspace_size(size_t batch, size_t d_model, size_t heads);
+size_t nsrl_decode_block_q4_workspace_size(const nsrl_q4_cache* cache);
 nsrl_status nsrl_prenorm_attention_decode_block_q4(const int16_t* x, size_t batch, size_t d_model, size_t heads,
                                                    const int16_t* rms_gamma, uint64_t rms_eps,
                                                    const nsrl_linear_params* q, const nsrl_linear_params* k,

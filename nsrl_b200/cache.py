@@ -36,12 +36,14 @@ def _lib():
         L.nsrl_q4_cache_max_capacity.restype = sz
         L.nsrl_q4_cache_append.argtypes = [cp, vp, vp, sz, sz, vp, vp, vp, vp, vp]
         L.nsrl_q4_cache_read.argtypes = [cp, vp, sz, vp, vp, vp, vp]
-        L.nsrl_attention_decode_q4.argtypes = [vp, sz, cp, vp, vp, vp, vp]
+        L.nsrl_attention_decode_q4_workspace_size.restype = sz
+        L.nsrl_attention_decode_q4_workspace_size.argtypes = [cp]
+        L.nsrl_attention_decode_q4.argtypes = [vp, sz, cp, vp, vp, vp, sz, vp, vp]
         L.nsrl_q4_cache_evict_workspace_size.restype = sz
         L.nsrl_q4_cache_evict_workspace_size.argtypes = [cp, sz]
         L.nsrl_q4_cache_evict.argtypes = [cp, vp, vp, sz, sz, sz, vp, vp, vp, vp, sz, vp, vp]
         L.nsrl_decode_block_q4_workspace_size.restype = sz
-        L.nsrl_decode_block_q4_workspace_size.argtypes = [sz, sz, sz]
+        L.nsrl_decode_block_q4_workspace_size.argtypes = [cp]
         L.nsrl_prenorm_attention_decode_block_q4.argtypes = [vp, sz, sz, sz, vp, C.c_uint64, lp, lp, lp, lp,
                                                              C.POINTER(RotaryC), cp, vp, vp, vp, vp, sz, vp, vp]
         L._q4_bound = True
@@ -91,6 +93,10 @@ class Q4Cache:
         self._cols = H * self.head_dim
         self._c = Q4CacheC(*ptr, B, H, self.head_dim, cap)
         self._ref = C.byref(self._c)
+        # the attention's workspace (4 bytes a slot and a little, none for a small cache) lives as long as the cache
+        nbytes = _lib().nsrl_attention_decode_q4_workspace_size(self._ref)
+        self._ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        self._ws_ptr, self._ws_bytes = (self._ws.data_ptr() if nbytes else None), nbytes
 
     def c(self) -> Q4CacheC:
         return self._c
@@ -139,7 +145,7 @@ class Q4Cache:
             raise core.NsrlError("q must be [batch, heads * head_dim]")
         return _lib().nsrl_attention_decode_q4(qp, core._row_stride(q), self._ref, self._per_sequence(lens, "lens"),
                                                core._array(ctx, torch.int16, (self.batch, cols), self._dev, "ctx"),
-                                               status.buf.data_ptr(), stream)
+                                               self._ws_ptr, self._ws_bytes, status.buf.data_ptr(), stream)
 
     def evict_workspace_bytes(self, keep: int) -> int:
         return _lib().nsrl_q4_cache_evict_workspace_size(self._ref, keep)
@@ -205,7 +211,7 @@ def prenorm_attention_decode_block_q4(x, rms_gamma, rms_eps, q, k, v, o, cache: 
     lp = cache._per_sequence(lens, "lens")
     pp = None if positions is None else cache._per_sequence(positions, "positions")
     y = torch.empty_like(x)
-    ws = core.workspace(L.nsrl_decode_block_q4_workspace_size(B, d, cache.heads))
+    ws = core.workspace(L.nsrl_decode_block_q4_workspace_size(cache._ref))
     st = core.Status()
     ps = [l.c() for l in (q, k, v, o)]
     h = core._run(lambda: L.nsrl_prenorm_attention_decode_block_q4(

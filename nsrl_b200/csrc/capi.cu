@@ -938,14 +938,23 @@ nsrl_status nsrl_q4_cache_read(const nsrl_q4_cache* cache, const int32_t* starts
   return NSRL_OK;
 }
 
+size_t nsrl_attention_decode_q4_workspace_size(const nsrl_q4_cache* cache) {
+  return check_q4(cache) == NSRL_OK ? q4_attend_workspace(*cache) : 0;
+}
+
 nsrl_status nsrl_attention_decode_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache* cache, const int32_t* lens,
-                                     int16_t* ctx, nsrl_device_status* status, void* stream) {
+                                     int16_t* ctx, void* workspace, size_t workspace_bytes,
+                                     nsrl_device_status* status, void* stream) {
   const nsrl_status r = check_q4(cache);
   if (r != NSRL_OK) return r;
   if (ldq < cache->heads * cache->head_dim) return shape_fail("q rows shorter than heads * head_dim");
   if (cache->batch == 0) return NSRL_OK;
   if (!q || !lens || !ctx || !status) return shape_fail("NULL argument");
-  NSRL_TRY(launch_attend_q4(q, ldq, *cache, lens, 0, ctx, status, (cudaStream_t)stream), "q4 decode attention");
+  const size_t need = q4_attend_workspace(*cache);
+  if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
+    return shape_fail("workspace too small or not 256-byte aligned");
+  NSRL_TRY(launch_attend_q4(q, ldq, *cache, lens, 0, ctx, workspace, status, (cudaStream_t)stream),
+           "q4 decode attention");
   return NSRL_OK;
 }
 
@@ -974,13 +983,15 @@ nsrl_status nsrl_q4_cache_evict(const nsrl_q4_cache* cache, const int32_t* lens,
   return NSRL_OK;
 }
 
-size_t nsrl_decode_block_q4_workspace_size(size_t batch, size_t d_model, size_t heads) {
-  (void)heads;
+size_t nsrl_decode_block_q4_workspace_size(const nsrl_q4_cache* cache) {
+  if (check_q4(cache) != NSRL_OK) return 0;
+  const size_t batch = cache->batch, d = cache->heads * cache->head_dim;
   Carver c(nullptr);
-  c.planes(batch, d_model, true);
-  c.take<int16_t>(batch * 3 * d_model);
-  c.take<int16_t>(batch * d_model);
-  c.planes(batch, d_model, true);
+  c.planes(batch, d, true);
+  c.take<int16_t>(batch * 3 * d);
+  c.take<int16_t>(batch * d);
+  c.planes(batch, d, true);
+  c.take<uint8_t>(q4_attend_workspace(*cache));
   return c.off;
 }
 
@@ -1004,8 +1015,8 @@ nsrl_status nsrl_prenorm_attention_decode_block_q4(const int16_t* x, size_t batc
   }
   if (batch == 0) return NSRL_OK;
   if (!x || !y || !status || !rms_gamma || !lens) return shape_fail("NULL argument");
-  if (!workspace || workspace_bytes < nsrl_decode_block_q4_workspace_size(batch, d_model, heads))
-    return shape_fail("workspace too small");
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < nsrl_decode_block_q4_workspace_size(cache))
+    return shape_fail("workspace too small or not 256-byte aligned");
   cudaStream_t s = (cudaStream_t)stream;
   const size_t d = d_model, hd = cache->head_dim;
   Carver c(workspace);
@@ -1013,6 +1024,7 @@ nsrl_status nsrl_prenorm_attention_decode_block_q4(const int16_t* x, size_t batc
   int16_t* qkv = c.take<int16_t>(batch * 3 * d);
   int16_t* ctx16 = c.take<int16_t>(batch * d);
   Planes ctx = c.planes(batch, d, true);
+  uint8_t* scratch = c.take<uint8_t>(q4_attend_workspace(*cache));
   if (!needs_l1(d, q, k, v)) xn.l1 = nullptr;
   if (!needs_l1(d, o)) ctx.l1 = nullptr;
   NSRL_TRY(launch_rms_norm(x, batch, d, rms_gamma, rms_eps, nullptr, xn, status, s), "rms norm");
@@ -1039,7 +1051,7 @@ nsrl_status nsrl_prenorm_attention_decode_block_q4(const int16_t* x, size_t batc
   NSRL_TRY(launch_q4_append(*cache, qkv + d, qkv + 2 * d, 3 * d, 1, lens, nullptr, positions ? positions : lens, status,
                             s),
            "q4 append");
-  NSRL_TRY(launch_attend_q4(qkv, 3 * d, *cache, lens, 1, ctx16, status, s), "q4 decode attention");
+  NSRL_TRY(launch_attend_q4(qkv, 3 * d, *cache, lens, 1, ctx16, scratch, status, s), "q4 decode attention");
   NSRL_TRY(launch_split_planes(ctx16, batch, d, d, ctx, s), "split planes");
   GemmArgs og{};
   og.a_hi = ctx.hi;

@@ -7,27 +7,32 @@
 //   sum p v = sum_j p_j zero_jg + (p_j scale_jg) code_j.
 //
 // The Q15 weights need the row's maximum and sum before the first value is
-// weighed, so a (sequence, head) is one cluster of CTAs: each takes a
-// contiguous share of the slots, keeps their logits in shared memory, and the
-// cluster exchanges maximum, sum and partial contexts through distributed
-// shared memory (maximum and sum by a store and an arrival on every CTA's own
-// barrier, so that the copying warp takes no part).  The cache is read once.
+// weighed.  Two forms, both of which read the cache once:
+//   WHOLE   one launch; a (sequence, head) is one CTA, or a cluster of them
+//           where rows are few: each takes a contiguous share of the slots,
+//           keeps their logits in shared memory, and the cluster exchanges
+//           maximum, sum and partial contexts through distributed shared memory.
+//   split   three launches over fixed chunks of slots: KEYS writes logits (4
+//           bytes a slot) and each chunk's maximum, sums_kernel each chunk's
+//           sum, VALUES each chunk's context; the last chunk of a row to arrive
+//           adds them up (integers: in any order the same).  No CTA waits for
+//           another, and chunks spread evenly over the SMs.
 //
 // Bound by memory (80 bytes a slot of 64 dims, 88 with scores) while an SM
-// spends less than about 3.5 cycles on a slot, so instructions are counted:
-//   keys:   a lane owns a slot; codes widen to bytes and meet the query's high
-//           (signed) and low (unsigned) byte planes in dp4a, 32 a slot.
-//   values: int8 MMAs (m16n8k32): A = 16 dims x 32 slots (a 4 x 4 byte
-//           transpose by PRMT), B = the four byte planes of p_j scale_jg of two
-//           groups, one column each.  An MMA takes 32 cycles of its quarter SM,
-//           one cycle a slot in all; for the keys, whose products need no
-//           transpose, dp4a costs fewer instructions.
-// Everything is exact in s32 until it is combined in 64 bits.  Two warps
-// stream tiles of codes and scales (K, then V) through a ring of bulk copies,
-// so value tiles arrive while the softmax runs (waiting for a stage and
-// refilling it takes a warp about 375 cycles whatever the size, more than a
-// tile's share of the memory's time: hence two).  Teams of consumer warps take
-// the tiles in turn, so that one team's latencies hide behind the others'.
+// spends less than about 3.5 cycles on a slot, that is some 14 instructions of
+// a warp on 32 slots each cycle it has; the integer pipes take one every other
+// cycle.  So instructions are counted:
+//   keys:   a lane owns a slot and loads its whole row; codes widen to bytes and
+//           meet the query's high (signed) and low (unsigned) byte planes in
+//           dp4a, 32 a slot.
+//   values: int8 MMAs (m16n8k32): A = 16 dims x 32 slots (transposing matrix
+//           loads from a kilobyte that the warp has to itself, and a PRMT), B =
+//           the four byte planes of p_j scale_jg of two groups, one column each.
+// Warps work on units of 32 slots by themselves, the next unit's loads under
+// way: a ring of bulk copies between warps cost as many instructions in waits
+// and index arithmetic as the products themselves (keys of 32 rows of 8,192
+// slots: 174 instructions a unit and 18 us even without the loads).
+// Everything is exact in s32 until it is combined in 64 bits.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -40,11 +45,11 @@ namespace cg = cooperative_groups;
 namespace nsrl {
 namespace {
 
-constexpr int WARPS = 16, COPIERS = 2;
-constexpr int CONSUMERS = 32 * WARPS, THREADS = CONSUMERS + 32 * COPIERS;
 constexpr int MAX_CLUSTER = 16;
-constexpr int SHARE_UNIT = 32;       // slots of a value MMA
+constexpr int UNIT = 32;             // slots of a warp's step
 constexpr size_t MAX_SHARE = 32768;  // logits of a CTA: 128 KB
+constexpr int CHUNK = 2048;          // slots of a CTA of the split form
+constexpr size_t SPLIT_BYTES = 24u << 20;  // cache bytes from which a call takes the split form
 
 template <int HD>
 struct Q4Shape {
@@ -53,13 +58,6 @@ struct Q4Shape {
   static constexpr int GW = HD < 32 ? HD / 8 : 4;  // code words of a group
   static constexpr int PAIRS = (G + 1) / 2;        // pairs of groups, 64 dims each
   static constexpr int SHIFT = HD == 16 ? 2 : HD == 64 ? 3 : 4;
-  static constexpr int TILE = HD == 16 ? 512 : HD == 64 ? 256 : 128;  // slots of a stage
-  static constexpr int TEAM = HD == 256 ? 4 : 8;                      // warps that share a tile
-  static constexpr int TEAMS = WARPS / TEAM;
-  static constexpr int STAGES = 4;
-  static constexpr int CODE_BYTES = TILE * HD / 2, SCALE_BYTES = TILE * G * 4;
-  static constexpr int STAGE_BYTES = CODE_BYTES + SCALE_BYTES;
-  static constexpr int Q_STRIDE = 4 * GW + 4;  // query words of a group in shared memory, padded against conflicts
 };
 
 struct AttendArgs {
@@ -70,52 +68,14 @@ struct AttendArgs {
   int len_offset;
   int16_t* ctx;
   nsrl_device_status* st;
+  // the split form's scratch
+  int chunks;           // of a row of `capacity` slots
+  int32_t* logits;      // [batch * heads][capacity]
+  int32_t* chunk_max;   // [batch * heads][chunks]
+  unsigned* chunk_sum;  // [batch * heads][chunks]
+  unsigned* arrived;    // [batch * heads]: chunks whose context is written
+  long long* partial;   // [batch * heads][chunks][head_dim]
 };
-
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory"); }
-
-// Untiled bulk copy global -> shared, both 16-byte aligned, a multiple of 16 bytes.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0, %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(20000u)
-      : "memory");
-  return ok != 0;
-}
-
-// Gives `value` to slot `part` of every CTA of the cluster and waits (bounded)
-// until all `parts` values are here.  All consumer threads call it with the
-// same arguments; thread r serves rank r.
-template <typename T>
-__device__ __forceinline__ bool exchange(const cg::cluster_group& cluster, T* values, uint64_t* bar, T value, int part,
-                                         int parts, nsrl_device_status* st) {
-  if ((int)threadIdx.x < parts) {
-    cluster.map_shared_rank(values, threadIdx.x)[part] = value;
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(bar)), "r"(threadIdx.x));
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
-  }
-  if (try_wait_cluster(bar)) return true;
-  const unsigned long long t0 = global_ns();
-  for (uint32_t i = 0;; ++i) {
-    if (try_wait_cluster(bar)) return true;
-    if ((i & 15u) == 15u && global_ns() - t0 > NSRL_WAIT_NS) {
-      nsrl_flag(st, NSRL_FLAG_WAIT_TIMEOUT);
-      return false;
-    }
-  }
-}
 
 __device__ __forceinline__ int dp4a_us(uint32_t a, uint32_t b, int c) {  // unsigned x signed bytes
   int d;
@@ -164,228 +124,23 @@ __device__ __forceinline__ unsigned weight(const int16_t* lut, int lg, int mx) {
   return (unsigned)lut[mag & 255] >> (mag >> 8);
 }
 
-template <int HD>
-__global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(const AttendArgs a) {
-  using S = Q4Shape<HD>;
-  extern __shared__ __align__(128) uint8_t dyn[];
-  int32_t* const logits = reinterpret_cast<int32_t*>(dyn + S::STAGES * S::STAGE_BYTES);
-  __shared__ uint64_t full[S::STAGES], empty[S::STAGES];
-  __shared__ uint64_t exchanged[2];  // the cluster's maxima and sums are here
-  __shared__ int16_t lut[256];
-  __shared__ uint32_t recip[128];
-  // per group and code word {h of the even dims, h of the odd dims, l even, l odd}; then 16 times the group's sum of q
-  __shared__ __align__(16) uint32_t s_q[S::G * S::Q_STRIDE];
-  __shared__ int s_max[MAX_CLUSTER], s_redi[WARPS];
-  __shared__ unsigned s_red[WARPS];
-  __shared__ unsigned long long s_sum[MAX_CLUSTER];
-  __shared__ long long s_part[WARPS / S::PAIRS][HD], s_ctx[HD];
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == CONSUMERS) {  // the copying warps do not wait for the others
-    for (int s = 0; s < S::STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], S::TEAM);
-    }
-    mbar_init(&exchanged[0], (uint32_t)parts);
-    mbar_init(&exchanged[1], (uint32_t)parts);
-    fence_barrier_init();
-  }
-  if (tid < 256)
-    lut[tid] = d_exp2_lut[tid];
-  else if (tid < 256 + 128)
-    recip[tid - 256] = d_recip_lut[tid - 256];
-  griddep_wait();
-  griddep_launch();
-  const unsigned bh = blockIdx.x / (unsigned)parts;
-  const unsigned b = bh / (unsigned)a.c.heads, h = bh - b * (unsigned)a.c.heads;
-  int q8[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (tid < S::WORDS) {
-    const int16_t* qp = a.q + b * a.ldq + (long long)h * HD + 8 * tid;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q8[i] = qp[i];
-  }
-  const long long len = (long long)a.lens[b] + a.len_offset;
-  if (len <= 0 || len > (long long)a.c.capacity) {  // the same for the whole cluster
-    if (tid == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
-    return;
-  }
-  const int share = ((int)((len + parts - 1) / parts) + SHARE_UNIT - 1) / SHARE_UNIT * SHARE_UNIT;
-  const long long first = (long long)part * share;
-  const int n = (int)max(0ll, min((long long)share, len - first));
-  const size_t slot0 = (size_t)bh * a.c.capacity + (size_t)first;
-  const int tiles = (n + S::TILE - 1) / S::TILE;
+// recip_sum_q31 with the table in shared memory.  Where any logit counts, the
+// slot at the maximum weighs 32767, so the sum is at least that (it is smaller
+// only after a timeout), the result at most 65793.
+__device__ __forceinline__ unsigned reciprocal(const uint32_t* recip, unsigned long long sum) {
+  if (sum < 32767) return 0;
+  const int shift = 63 - __clzll((long long)sum) - 7;
+  return recip[((unsigned)(sum >> shift) & 255u) - 128] >> shift;
+}
 
-  if (warp >= WARPS) {
-    // ---------------------------------------------------------------- copies
-    if (parts > 1) {
-      cluster.sync();  // every CTA's barriers are ready
-    } else {
-      asm volatile("bar.sync 3, %0;" ::"n"(32 * COPIERS) : "memory");
-      asm volatile("bar.arrive 2, %0;" ::"n"(THREADS) : "memory");
-    }
-    if (lane == 0) {
-      static_assert(S::STAGES % COPIERS == 0);
-      int issued = 0;
-      for (int it = warp - WARPS; it < 2 * tiles; it += COPIERS) {
-        const int s = it % S::STAGES;
-        if (it >= S::STAGES && !mbar_wait(&empty[s], ((it / S::STAGES) - 1) & 1, a.st)) break;
-        const bool value = it >= tiles;
-        const int at = (value ? it - tiles : it) * S::TILE;
-        // whole 16-slot runs: a multiple of 16 bytes, and inside the capacity
-        const uint32_t slots = (uint32_t)(min(S::TILE, n - at) + 15) & ~15u;
-        uint8_t* stage = dyn + s * S::STAGE_BYTES;
-        mbar_arrive_expect_tx(&full[s], slots * (HD / 2 + 4 * S::G));
-        bulk_load(stage, (value ? a.c.v_codes : a.c.k_codes) + (slot0 + at) * (HD / 2), slots * (HD / 2), &full[s]);
-        bulk_load(stage + S::CODE_BYTES, (value ? a.c.v_scales : a.c.k_scales) + (slot0 + at) * S::G, slots * 4 * S::G,
-                  &full[s]);
-        issued = it + 1;
-      }
-      // the copies in flight land before the CTA may leave: this warp's last ones, one a stage
-      for (int it = issued - 1; it >= 0 && it > issued - 1 - S::STAGES; it -= COPIERS)
-        mbar_wait(&full[it % S::STAGES], (it / S::STAGES) & 1, a.st);
-    }
-    __syncwarp();
-    if (parts > 1) {
-      cluster.sync();
-      cluster.sync();
-    }
-    return;
-  }
-
-  if (tid < S::WORDS) {
-    uint32_t w[4] = {0, 0, 0, 0};
-    int sum = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum += q8[i];
-      w[i & 1] |= (uint32_t)((q8[i] >> 8) & 255) << (8 * (i >> 1));
-      w[2 + (i & 1)] |= (uint32_t)(q8[i] & 255) << (8 * (i >> 1));
-    }
-    const unsigned mask = S::WORDS >= 32 ? 0xffffffffu : (1u << S::WORDS) - 1;
-#pragma unroll
-    for (int o = 1; o < S::GW; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
-    uint32_t* group = s_q + (tid / S::GW) * S::Q_STRIDE;
-    *reinterpret_cast<uint4*>(group + 4 * (tid % S::GW)) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (tid % S::GW == 0) group[4 * S::GW] = (uint32_t)(16 * sum);
-  }
-  if (parts > 1)
-    cluster.sync();
-  else
-    asm volatile("bar.sync 2, %0;" ::"n"(THREADS) : "memory");
-
-  // -------------------------------------------------------------------- keys
-  // A lane's slot is r + lane.  Lanes of 256-dim slots (128 bytes apart) start
-  // at different groups, so that no two of a load meet in a bank.
-  const int team = warp / S::TEAM, mate = warp % S::TEAM;
-  constexpr bool HELD = S::G <= 2;  // the query's words in registers
-  uint4 qw[HELD ? S::WORDS : 1];
-  int qs[HELD ? S::G : 1];
-  if constexpr (HELD) {
-#pragma unroll
-    for (int i = 0; i < S::G; ++i) qs[i] = (int)s_q[i * S::Q_STRIDE + 4 * S::GW];
-#pragma unroll
-    for (int i = 0; i < S::WORDS; ++i)
-      qw[i] = *reinterpret_cast<const uint4*>(s_q + (i / S::GW) * S::Q_STRIDE + 4 * (i % S::GW));
-  }
-  bool bad = false, alive = true;
-  int mx = INT_MIN;
-  for (int it = team; it < tiles && alive; it += S::TEAMS) {
-    const int s = it % S::STAGES;
-    alive = mbar_wait(&full[s], (it / S::STAGES) & 1, a.st);
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(dyn + s * S::STAGE_BYTES);
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(dyn + s * S::STAGE_BYTES + S::CODE_BYTES);
-    const int left = n - it * S::TILE;
-    constexpr int UNITS = S::TILE / (32 * S::TEAM);
-    // The rows go to registers first, where they fit, and the stage back to the copies.
-    uint32_t held[HELD ? UNITS : 1][HELD ? S::WORDS : 1], held_scale[HELD ? UNITS : 1][HELD ? S::G : 1];
-    if constexpr (HELD) {
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int slot = 32 * (u * S::TEAM + mate) + lane;
-        const uint32_t* row = codes + slot * S::WORDS;
-        if constexpr (HD == 16) {
-          const uint2 x = *reinterpret_cast<const uint2*>(row);
-          held[u][0] = x.x, held[u][1] = x.y;
-          held_scale[u][0] = scales[slot];
-        } else {
-#pragma unroll
-          for (int i = 0; i < S::WORDS; i += 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(row + i);
-            held[u][i] = x.x, held[u][i + 1] = x.y, held[u][i + 2] = x.z, held[u][i + 3] = x.w;
-          }
-          const uint2 x = *reinterpret_cast<const uint2*>(scales + 2 * slot);
-          held_scale[u][0] = x.x, held_scale[u][1] = x.y;
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
-    }
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int slot = 32 * (u * S::TEAM + mate) + lane;
-      if (slot - lane >= left) break;
-      long long v = 0;
-#pragma unroll
-      for (int i = 0; i < S::G; ++i) {
-        const int c = HELD ? i : (i + lane) % S::G;
-        uint32_t w[S::GW], sw;
-        if constexpr (HELD) {
-#pragma unroll
-          for (int k = 0; k < S::GW; ++k) w[k] = held[u][S::GW * i + k];
-          sw = held_scale[u][i];
-        } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(codes + slot * S::WORDS + 4 * c);
-          w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-          sw = scales[slot * S::G + c];
-        }
-        // odd dims stay in the high half bytes, 16 times over: the even dims' sums catch up
-        int he = 0, ho = 0, le = 0, lo = 0;
-#pragma unroll
-        for (int k = 0; k < S::GW; ++k) {
-          const uint4 q = HELD ? qw[S::GW * i + k] : *reinterpret_cast<const uint4*>(s_q + c * S::Q_STRIDE + 4 * k);
-          he = dp4a_us(w[k] & LOW, q.x, he);
-          ho = dp4a_us(w[k] & HIGH, q.y, ho);
-          le = dp4a_uu(w[k] & LOW, q.z, le);
-          lo = dp4a_uu(w[k] & HIGH, q.w, lo);
-        }
-        const int dot = (he * 256 + le) * 16 + (ho * 256 + lo);  // 16 sum q code, below 2^28
-        const int qsum = HELD ? qs[i] : (int)s_q[c * S::Q_STRIDE + 4 * S::GW];
-        v += (long long)dot * (int)(sw & 0xFFFF) + (long long)qsum * ((int)sw >> 16);
-      }
-      if (slot < left) {
-        const long long lg = v >> (S::SHIFT + 4);
-        bad = bad || lg != (long long)(int)lg;
-        logits[it * S::TILE + slot] = (int)lg;
-        mx = max(mx, (int)lg);  // MASKED_LOGIT is INT_MIN: it never raises the maximum
-      }
-    }
-    if constexpr (!HELD) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
-    }
-  }
-  if (bad) nsrl_flag(a.st, NSRL_FLAG_LOGIT_RANGE);
-  mx = __reduce_max_sync(0xffffffffu, mx);
-  if (lane == 0) s_redi[warp] = mx;
-  consumers_sync();
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) mx = max(mx, s_redi[w]);
-  if (parts > 1) {
-    alive = exchange(cluster, s_max, &exchanged[0], mx, part, parts, a.st) && alive;
-    for (int r = 0; r < parts; ++r) mx = max(mx, s_max[r]);
-  }
-  const bool any = mx != INT_MIN;
-  if (!any && tid == 0 && part == 0) nsrl_flag(a.st, NSRL_FLAG_ALL_MASKED);
-
-  // ---------------------------------------------------------------- softmax
-  // Only the sum: the value pass weighs each slot again.  A CTA's sum is at most
-  // 2^15 * MAX_SHARE = 2^30.
-  unsigned part_sum = 0;
+// The sum of weight() over n logits at `logits` (16-byte aligned), this thread's part.
+template <int THREADS>
+__device__ __forceinline__ unsigned weigh(const int16_t* lut, const int32_t* logits, int n, int mx) {
+  unsigned sum = 0;
   const bool low = mx < INT_MIN + 15 * 256;  // MASKED_LOGIT would gather weight
   const int none = (int)((unsigned)mx - 15u * 256u);
 #pragma unroll 2
-  for (int j = 4 * tid; j < n; j += 4 * CONSUMERS) {
+  for (int j = 4 * (int)threadIdx.x; j < n; j += 4 * THREADS) {
     int4 lg = *reinterpret_cast<const int4*>(logits + j);
     if (j + 3 >= n || low) {
       if (lg.x == INT_MIN) lg.x = none;
@@ -393,39 +148,198 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
       if (lg.z == INT_MIN || j + 2 >= n) lg.z = none;
       if (lg.w == INT_MIN || j + 3 >= n) lg.w = none;
     }
-    part_sum += weight(lut, lg.x, mx) + weight(lut, lg.y, mx) + weight(lut, lg.z, mx) + weight(lut, lg.w, mx);
+    sum += weight(lut, lg.x, mx) + weight(lut, lg.y, mx) + weight(lut, lg.z, mx) + weight(lut, lg.w, mx);
   }
-  part_sum = __reduce_add_sync(0xffffffffu, part_sum);
-  if (lane == 0) s_red[warp] = part_sum;
-  consumers_sync();
-  unsigned long long sum = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) sum += s_red[w];
-  if (parts > 1) {
-    alive = exchange(cluster, s_sum, &exchanged[1], sum, part, parts, a.st) && alive;
-    sum = 0;
-    for (int r = 0; r < parts; ++r) sum += s_sum[r];
-  }
-  // The slot at the maximum has weight 32767, so sum >= 32767, inv <= 65793 and
-  // w inv + 2^15 < 2^32: sat_i16(rhu64(w * inv, 16)) in 32 bits.
-  unsigned inv = 0;
-  if (any && sum >= 32767) {  // recip_sum_q31, the table in shared memory (the sum is smaller only after a timeout)
-    const int shift = 63 - __clzll((long long)sum) - 7;
-    inv = recip[((unsigned)(sum >> shift) & 255u) - 128] >> shift;
-  }
+  return sum;
+}
 
-  // ------------------------------------------------------------------ values
-  // A warp's unit is 32 slots of one pair of groups (64 dims).  Transposing
-  // matrix loads give lane (g, t) bytes 2 g and 2 g + 1 of a group's row for
-  // slots 8 m + 2 t and 8 m + 2 t + 1; two loads and a PRMT make one byte of four
-  // slots.  16 dims a head (8-byte rows): byte g of slots 4 j + t from words.  A
-  // byte holds an even and an odd dim: row g of its MMA takes the byte as it is
-  // (even + 16 odd), row g + 8 its high half (16 odd), and they part at the
-  // end.  Slot `own` is this lane's to weigh (p, its score, p scale: 0 past the share); the
-  // byte planes of p scale then go to the lanes of their column.
+// ---------------------------------------------------------------------- keys
+// The query of one (sequence, head) in shared memory: per group and code word
+// {h of the even dims, h of the odd dims, l even, l odd} with q = 256 h + l, then
+// 16 times the group's sum of q.
+template <int HD>
+struct Query {
+  uint4 word[Q4Shape<HD>::WORDS];
+  int sum16[Q4Shape<HD>::G];
+};
+
+// Warp 0 lays it out; the caller synchronises.
+template <int HD>
+__device__ __forceinline__ void lay_out(Query<HD>& q, const int16_t* row) {
+  using S = Q4Shape<HD>;
+  const int lane = threadIdx.x;
+  if (lane >= S::WORDS) return;
+  uint32_t w[4] = {0, 0, 0, 0};
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int v = row[8 * lane + i];
+    sum += v;
+    w[i & 1] |= (uint32_t)((v >> 8) & 255) << (8 * (i >> 1));
+    w[2 + (i & 1)] |= (uint32_t)(v & 255) << (8 * (i >> 1));
+  }
+  constexpr unsigned mask = S::WORDS >= 32 ? 0xffffffffu : (1u << S::WORDS) - 1;
+#pragma unroll
+  for (int o = 1; o < S::GW; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
+  q.word[lane] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (lane % S::GW == 0) q.sum16[lane / S::GW] = 16 * sum;
+}
+
+// A slot's row of codes and scales.
+template <int HD>
+struct KeyRow {
+  uint32_t code[Q4Shape<HD>::WORDS];
+  uint32_t scale[Q4Shape<HD>::G];
+
+  __device__ __forceinline__ void load(const nsrl_q4_cache& c, size_t slot) {
+    const uint8_t* p = c.k_codes + slot * (HD / 2);
+    const uint32_t* s = c.k_scales + slot * Q4Shape<HD>::G;
+    if constexpr (HD == 16) {
+      const uint2 x = __ldcs(reinterpret_cast<const uint2*>(p));
+      code[0] = x.x, code[1] = x.y;
+      scale[0] = __ldcs(s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < Q4Shape<HD>::WORDS; i += 4) {
+        const uint4 x = __ldcs(reinterpret_cast<const uint4*>(p) + i / 4);
+        code[i] = x.x, code[i + 1] = x.y, code[i + 2] = x.z, code[i + 3] = x.w;
+      }
+#pragma unroll
+      for (int i = 0; i < Q4Shape<HD>::G; i += 2) {
+        const uint2 x = __ldcs(reinterpret_cast<const uint2*>(s) + i / 2);
+        scale[i] = x.x, scale[i + 1] = x.y;
+      }
+    }
+  }
+};
+
+// 16 q . k of R slots (odd dims stay in the high half bytes, the even ones
+// catch up); the query's words are read once for all of them.
+template <int HD, int R>
+__device__ __forceinline__ void dots16(const Query<HD>& query, const KeyRow<HD> (&row)[R], long long (&v)[R]) {
+  using S = Q4Shape<HD>;
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = 0;
+#pragma unroll
+  for (int g = 0; g < S::G; ++g) {
+    int he[R], ho[R], le[R], lo[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) he[r] = ho[r] = le[r] = lo[r] = 0;
+#pragma unroll
+    for (int k = 0; k < S::GW; ++k) {
+      const uint4 q = query.word[S::GW * g + k];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint32_t w = row[r].code[S::GW * g + k];
+        he[r] = dp4a_us(w & LOW, q.x, he[r]);
+        ho[r] = dp4a_us(w & HIGH, q.y, ho[r]);
+        le[r] = dp4a_uu(w & LOW, q.z, le[r]);
+        lo[r] = dp4a_uu(w & HIGH, q.w, lo[r]);
+      }
+    }
+    const int sum16 = query.sum16[g];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int dot = (he[r] * 256 + le[r]) * 16 + (ho[r] * 256 + lo[r]);  // 16 sum q code, below 2^28
+      v[r] += (long long)dot * (int)(row[r].scale[g] & 0xFFFF) + (long long)sum16 * ((int)row[r].scale[g] >> 16);
+    }
+  }
+}
+
+// Logits of n slots from slot0; returns this warp's maximum (INT_MIN: none
+// counts; MASKED_LOGIT is INT_MIN and never raises it).  A step takes R units,
+// the next step's rows under way where registers allow.
+template <int HD, int WARPS>
+__device__ __forceinline__ int keys_pass(const AttendArgs& a, const Query<HD>& query, size_t slot0, int n,
+                                         int32_t* logits) {
+  using S = Q4Shape<HD>;
+  constexpr int R = HD == 256 ? 1 : 2, APART = UNIT * WARPS;
+  constexpr bool AHEAD = HD != 256;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int mx = INT_MIN;
+  bool bad = false;
+  KeyRow<HD> row[R], next[AHEAD ? R : 1];
+  int j = UNIT * warp + lane;
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (j + r * APART < n) next[r].load(a.c, slot0 + j + r * APART);
+  }
+  for (; j < n; j += R * APART) {
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) row[r] = next[r];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (j + (R + r) * APART < n) next[r].load(a.c, slot0 + j + (R + r) * APART);
+    } else {
+      row[0].load(a.c, slot0 + j);
+    }
+    long long v[R];
+    dots16<HD, R>(query, row, v);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (j + r * APART >= n) break;
+      const long long lg = v[r] >> (S::SHIFT + 4);
+      bad = bad || lg != (long long)(int)lg;
+      logits[j + r * APART] = (int)lg;
+      mx = max(mx, (int)lg);
+    }
+  }
+  if (bad) nsrl_flag(a.st, NSRL_FLAG_LOGIT_RANGE);
+  return __reduce_max_sync(0xffffffffu, mx);
+}
+
+// -------------------------------------------------------------------- values
+// A warp's unit is 32 slots of one pair of groups (64 dims).  Transposing
+// matrix loads give lane (g, t) bytes 2 g and 2 g + 1 of a group's row for
+// slots 8 m + 2 t and 8 m + 2 t + 1; two of them and a PRMT make one byte of
+// four slots.  16 dims a head (8-byte rows): byte g of slots 4 j + t from words.
+// A byte holds an even and an odd dim: row g of its MMA takes the byte as it is
+// (even + 16 odd), row g + 8 its high half (16 odd), and they part at the end.
+// Slot `own` is this lane's to weigh (p, its score, p scale); the byte planes of
+// p scale then go to the lanes of their column.
+template <int HD>
+struct ValueUnit {
+  uint4 code[2];  // HD 16: the first 8 bytes
+  uint2 scale;
+  int logit, score;
+
+  // left: slots from the unit's first one to the end
+  __device__ __forceinline__ void load(const nsrl_q4_cache& c, size_t slot, int pair, int own, int left,
+                                       const int32_t* logits, const int32_t* scores) {
+    const int lane = threadIdx.x & 31;
+    // rows past the end are inside the capacity up to the next multiple of 16 slots
+    const int last = (left + 15) & ~15;
+    if constexpr (HD == 16) {
+      const uint2 x = lane < last ? __ldcs(reinterpret_cast<const uint2*>(c.v_codes) + slot + lane) : make_uint2(0, 0);
+      code[0].x = x.x, code[0].y = x.y;
+      scale = make_uint2(own < left ? __ldcs(c.v_scales + slot + own) : 0u, 0u);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 16 * e + (lane >> 1);
+        code[e] = r < last ? __ldcs(reinterpret_cast<const uint4*>(c.v_codes + (slot + r) * (HD / 2) + 32 * pair) + (lane & 1))
+                           : make_uint4(0, 0, 0, 0);
+      }
+      scale = own < left ? __ldcs(reinterpret_cast<const uint2*>(c.v_scales + (slot + own) * Q4Shape<HD>::G) + pair)
+                         : make_uint2(0, 0);
+    }
+    logit = own < left ? logits[own] : INT_MIN;
+    score = scores && own < left ? scores[own] : 0;
+  }
+};
+
+// Context of n slots from slot0 into part[HD] (this warp's row; only the pair's dims are written).
+template <int HD, int WARPS>
+__device__ __forceinline__ void values_pass(const AttendArgs& a, size_t slot0, int n, const int32_t* logits,
+                                            const int16_t* lut, int mx, unsigned inv, uint8_t* buffer,
+                                            long long* part) {
+  using S = Q4Shape<HD>;
   constexpr int MMAS = HD == 16 ? 1 : 4;
-  const int g = lane >> 2, t = lane & 3;
-  const int pair = mate % S::PAIRS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int pair = warp % S::PAIRS;
+  const int step = UNIT * (WARPS / S::PAIRS);
   int acc[MMAS][4];
 #pragma unroll
   for (int i = 0; i < MMAS; ++i)
@@ -437,88 +351,66 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
   const int from = 4 * t + (g & 3);  // the lane with plane g & 3 of the slots of k = 4 t; 16 further, of 16 + 4 t
   const uint32_t byte2 = (uint32_t)(g & 3) | ((uint32_t)((g & 3) + 4) << 4);  // byte g & 3 of two words
   int32_t* const scores = a.c.scores && pair == 0 ? a.c.scores + slot0 : nullptr;
-  // A stage stays with one team for both passes, so that no wait skips a phase.
-  static_assert(S::STAGES % S::TEAMS == 0);
-  for (int it = tiles + (team - tiles % S::TEAMS + S::TEAMS) % S::TEAMS; it < 2 * tiles && alive; it += S::TEAMS) {
-    const int s = it % S::STAGES;
-    const int at = (it - tiles) * S::TILE, left = n - at;
-    constexpr int STEP = S::TEAM / S::PAIRS, UNITS = S::TILE / 32 / STEP;
-    int old[UNITS];
-    if (scores) {
-#pragma unroll
-      for (int k = 0; k < UNITS; ++k) {
-        const int slot = 32 * (k * STEP + mate / S::PAIRS) + own;
-        old[k] = slot < left ? scores[at + slot] : 0;
-      }
-    }
-    alive = mbar_wait(&full[s], (it / S::STAGES) & 1, a.st);
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(dyn + s * S::STAGE_BYTES);
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(dyn + s * S::STAGE_BYTES + S::CODE_BYTES);
-    uint32_t w[UNITS][8];
-    uint2 sw[UNITS];
-    auto load = [&](int k) {
-      const int r = 32 * (k * STEP + mate / S::PAIRS);
-      if constexpr (HD == 16) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[k][j] = codes[(r + 4 * j + t) * S::WORDS + (g >> 2)];
-        sw[k] = make_uint2(scales[r + own], 0);
-      } else {
-        // lane l points at row r + l; w[k][4 e + m] is group e of slots 8 m ..
-        const uint32_t row = smem_u32(codes + (r + lane) * S::WORDS + 8 * pair);
-        load_matrices(row, w[k]);
-        load_matrices(row + 16, w[k] + 4);
-        sw[k] = *reinterpret_cast<const uint2*>(scales + (r + own) * S::G + 2 * pair);
-      }
-    };
-    if constexpr (HD != 256) {
-#pragma unroll
-      for (int k = 0; k < UNITS; ++k) load(k);
+  // Rows of 32 bytes in the warp's buffer, the halves of rows 4 .. 7 of eight
+  // swapped so that the matrix loads' eight rows meet no bank twice.
+  const uint32_t store_at = smem_u32(buffer) + 32 * (lane >> 1) + 16 * ((lane & 1) ^ ((lane >> 3) & 1));
+  const uint32_t load_at = smem_u32(buffer) + 32 * lane + 16 * ((lane >> 2) & 1);
+  ValueUnit<HD> unit, next;
+  int r = UNIT * (warp / S::PAIRS);
+  if (r < n) next.load(a.c, slot0 + r, pair, own, n - r, logits + r, scores ? scores + r : nullptr);
+  for (; r < n; r += step) {
+    unit = next;
+    const int ahead = r + step;
+    if (ahead < n) next.load(a.c, slot0 + ahead, pair, own, n - ahead, logits + ahead, scores ? scores + ahead : nullptr);
+    const int p =
+        unit.logit == INT_MIN ? 0 : (int)min((weight(lut, unit.logit, mx) * inv + 32768u) >> 16, 32767u);
+    if (scores && r + own < n) scores[r + own] = add_sat(unit.score, p);
+    uint32_t w[8];
+    if constexpr (HD == 16) {
+      *reinterpret_cast<uint2*>(buffer + 8 * lane) = make_uint2(unit.code[0].x, unit.code[0].y);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
-    }
 #pragma unroll
-    for (int k = 0; k < UNITS; ++k) {
-      const int r = 32 * (k * STEP + mate / S::PAIRS);
-      if (r >= left) break;
-      if constexpr (HD == 256) load(k);
-      const int lg = logits[at + r + own];
-      const bool masked = r + own >= left || lg == INT_MIN;
-      const int p = masked ? 0 : (int)min((weight(lut, lg, mx) * inv + 32768u) >> 16, 32767u);
-      if (scores && r + own < left) scores[at + r + own] = add_sat(old[k], p);
-      uint32_t bf[2];
-      zero_part[0] += (long long)p * ((int)sw[k].x >> 16);
-      const uint32_t plane0 = quad_plane((uint32_t)p * (sw[k].x & 0xFFFF), t);
-      if constexpr (HD == 16) {
-        bf[0] = __shfl_sync(0xffffffffu, plane0, from);
-        bf[1] = __shfl_sync(0xffffffffu, plane0, from + 16);
-      } else {
-        zero_part[1] += (long long)p * ((int)sw[k].y >> 16);
-        const uint32_t plane1 = quad_plane((uint32_t)p * (sw[k].y & 0xFFFF), t);
+      for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const uint32_t*>(buffer + 8 * (4 * j + t) + 4 * (g >> 2));
+    } else {
 #pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          const uint32_t x = __shfl_sync(0xffffffffu, plane0, from + 16 * o);
-          const uint32_t y = __shfl_sync(0xffffffffu, plane1, from + 16 * o);
-          bf[o] = (g >> 2) ? y : x;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < MMAS; ++i) {
-        uint32_t x, y;  // the byte of k = 4 t .. and of k = 16 + 4 t ..
-        if constexpr (HD == 16) {
-          x = __byte_perm(__byte_perm(w[k][0], w[k][1], byte2), __byte_perm(w[k][2], w[k][3], byte2), 0x5410);
-          y = __byte_perm(__byte_perm(w[k][4], w[k][5], byte2), __byte_perm(w[k][6], w[k][7], byte2), 0x5410);
-        } else {  // MMA i: byte i & 1 of group i >> 1
-          const uint32_t* m = w[k] + 4 * (i >> 1);
-          x = __byte_perm(m[0], m[1], (i & 1) ? 0x7531 : 0x6420);
-          y = __byte_perm(m[2], m[3], (i & 1) ? 0x7531 : 0x6420);
-        }
-        const uint32_t frag[4] = {x, x & HIGH, y, y & HIGH};
-        mma_u8u8(acc[i], frag, bf);
-      }
-    }
-    if constexpr (HD == 256) {
+      for (int e = 0; e < 2; ++e)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(store_at + 512 * e), "r"(unit.code[e].x),
+                     "r"(unit.code[e].y), "r"(unit.code[e].z), "r"(unit.code[e].w)
+                     : "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
+      load_matrices(load_at, w);           // w[4 e + m]: group e of slots 8 m ..
+      load_matrices(load_at ^ 16, w + 4);
+    }
+    __syncwarp();
+    uint32_t bf[2];
+    zero_part[0] += (long long)p * ((int)unit.scale.x >> 16);
+    const uint32_t plane0 = quad_plane((uint32_t)p * (unit.scale.x & 0xFFFF), t);
+    if constexpr (HD == 16) {
+      bf[0] = __shfl_sync(0xffffffffu, plane0, from);
+      bf[1] = __shfl_sync(0xffffffffu, plane0, from + 16);
+    } else {
+      zero_part[1] += (long long)p * ((int)unit.scale.y >> 16);
+      const uint32_t plane1 = quad_plane((uint32_t)p * (unit.scale.y & 0xFFFF), t);
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const uint32_t x = __shfl_sync(0xffffffffu, plane0, from + 16 * o);
+        const uint32_t y = __shfl_sync(0xffffffffu, plane1, from + 16 * o);
+        bf[o] = (g >> 2) ? y : x;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MMAS; ++i) {
+      uint32_t x, y;  // the byte of k = 4 t .. and of k = 16 + 4 t ..
+      if constexpr (HD == 16) {
+        x = __byte_perm(__byte_perm(w[0], w[1], byte2), __byte_perm(w[2], w[3], byte2), 0x5410);
+        y = __byte_perm(__byte_perm(w[4], w[5], byte2), __byte_perm(w[6], w[7], byte2), 0x5410);
+      } else {  // MMA i: byte i & 1 of group i >> 1
+        const uint32_t* m = w + 4 * (i >> 1);
+        x = __byte_perm(m[0], m[1], (i & 1) ? 0x7531 : 0x6420);
+        y = __byte_perm(m[2], m[3], (i & 1) ? 0x7531 : 0x6420);
+      }
+      const uint32_t frag[4] = {x, x & HIGH, y, y & HIGH};
+      mma_u8u8(acc[i], frag, bf);
     }
   }
   // Columns 2 t and 2 t + 1 are planes 2 (t & 1) and 2 (t & 1) + 1 of group t >> 1
@@ -536,16 +428,88 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
       long long v = ((long long)p0 + ((long long)p1 << 8)) << (16 * (t & 1));
       v += __shfl_xor_sync(0xffffffffu, v, 1);
       const int dim = HD == 16 ? 2 * g + o : 64 * pair + 32 * (i >> 1) + 4 * g + 2 * (i & 1) + o;
-      if (t == 2 * (i >> 1)) s_part[warp / S::PAIRS][dim] = v + zero_part[i >> 1];
+      if (t == 2 * (i >> 1)) part[dim] = v + zero_part[i >> 1];
     }
-  consumers_sync();
+}
+
+// --------------------------------------------------------------- one launch
+constexpr int WHOLE_WARPS = 16, WHOLE_THREADS = 32 * WHOLE_WARPS;
+
+// Gives `value` to entry `part` of every CTA of the cluster; all of them are
+// here once the cluster has synchronised.
+template <typename T>
+__device__ __forceinline__ void share_out(const cg::cluster_group& cluster, T* values, T value, int part, int parts) {
+  if ((int)threadIdx.x < parts) cluster.map_shared_rank(values, threadIdx.x)[part] = value;
+  cluster.sync();
+}
+
+template <int HD>
+__global__ void __launch_bounds__(WHOLE_THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(const AttendArgs a) {
+  using S = Q4Shape<HD>;
+  extern __shared__ __align__(16) int32_t logits[];
+  __shared__ Query<HD> query;
+  __shared__ __align__(128) uint8_t buffer[WHOLE_WARPS][1024];
+  __shared__ int16_t lut[256];
+  __shared__ uint32_t recip[128];
+  __shared__ int s_max[MAX_CLUSTER], s_redi[WHOLE_WARPS];
+  __shared__ unsigned s_red[WHOLE_WARPS];
+  __shared__ unsigned long long s_sum[MAX_CLUSTER];
+  __shared__ long long s_part[WHOLE_WARPS / S::PAIRS][HD], s_ctx[HD];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < 256) lut[tid] = d_exp2_lut[tid];
+  if (tid < 128) recip[tid] = d_recip_lut[tid];
+  griddep_wait();
+  griddep_launch();
+  const unsigned bh = blockIdx.x / (unsigned)parts, b = bh / (unsigned)a.c.heads, h = bh - b * (unsigned)a.c.heads;
+  const long long len = (long long)a.lens[b] + a.len_offset;
+  if (warp == 0) lay_out<HD>(query, a.q + b * a.ldq + (long long)h * HD);
+  if (len <= 0 || len > (long long)a.c.capacity) {  // the same for the whole cluster
+    if (tid == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
+    return;
+  }
+  const int share = ((int)((len + parts - 1) / parts) + UNIT - 1) / UNIT * UNIT;
+  const long long first = (long long)part * share;
+  const int n = (int)max(0ll, min((long long)share, len - first));
+  const size_t slot0 = (size_t)bh * a.c.capacity + (size_t)first;
+  if (parts > 1)
+    cluster.sync();  // every CTA has started: its shared memory may be written
+  else
+    __syncthreads();
+
+  int mx = keys_pass<HD, WHOLE_WARPS>(a, query, slot0, n, logits);
+  if (lane == 0) s_redi[warp] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WHOLE_WARPS; ++w) mx = max(mx, s_redi[w]);
+  if (parts > 1) {
+    share_out(cluster, s_max, mx, part, parts);
+    for (int r = 0; r < parts; ++r) mx = max(mx, s_max[r]);
+  }
+  if (mx == INT_MIN && tid == 0 && part == 0) nsrl_flag(a.st, NSRL_FLAG_ALL_MASKED);
+  // Only the sum: the value pass weighs each slot again.  A CTA's sum is at most 2^15 * MAX_SHARE = 2^30.
+  const unsigned mine = __reduce_add_sync(0xffffffffu, weigh<WHOLE_THREADS>(lut, logits, n, mx));
+  if (lane == 0) s_red[warp] = mine;
+  __syncthreads();
+  unsigned long long sum = 0;
+#pragma unroll
+  for (int w = 0; w < WHOLE_WARPS; ++w) sum += s_red[w];
+  if (parts > 1) {
+    share_out(cluster, s_sum, sum, part, parts);
+    sum = 0;
+    for (int r = 0; r < parts; ++r) sum += s_sum[r];
+  }
+  const unsigned inv = mx == INT_MIN ? 0u : reciprocal(recip, sum);
+  values_pass<HD, WHOLE_WARPS>(a, slot0, n, logits, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
+  __syncthreads();
   long long total = 0;
   if (tid < HD) {
 #pragma unroll
-    for (int w = 0; w < WARPS / S::PAIRS; ++w) total += s_part[w][tid];
-    s_ctx[tid] = total;
+    for (int w = 0; w < WHOLE_WARPS / S::PAIRS; ++w) total += s_part[w][tid];
   }
   if (parts > 1) {
+    if (tid < HD) s_ctx[tid] = total;
     cluster.sync();
     if (part == 0 && tid < HD)
       for (int r = 1; r < parts; ++r) total += cluster.map_shared_rank(s_ctx, r)[tid];
@@ -555,12 +519,137 @@ __global__ void __launch_bounds__(THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(c
   if (parts > 1) cluster.sync();  // no CTA leaves while rank 0 reads its partial context
 }
 
+// ------------------------------------------------------------ three launches
+// Grids are (batch * heads, chunks): a CTA is one chunk of one row.
+constexpr int SPLIT_WARPS = 8, SPLIT_THREADS = 32 * SPLIT_WARPS;
+
+// A chunk's place: false past the row's end (or for a bad length, which KEYS flags).
+struct Chunk {
+  unsigned bh, b, h;
+  int n, live;  // slots; chunks of the row
+  size_t slot0;
+  long long len;
+
+  __device__ __forceinline__ bool find(const AttendArgs& a) {
+    bh = blockIdx.x;
+    b = bh / (unsigned)a.c.heads;
+    h = bh - b * (unsigned)a.c.heads;
+    len = (long long)a.lens[b] + a.len_offset;
+    if (len <= 0 || len > (long long)a.c.capacity) return false;
+    const long long first = (long long)blockIdx.y * CHUNK;
+    if (first >= len) return false;
+    n = (int)min((long long)CHUNK, len - first);
+    live = (int)((len + CHUNK - 1) / CHUNK);
+    slot0 = (size_t)bh * a.c.capacity + (size_t)first;
+    return true;
+  }
+};
+
 template <int HD>
-cudaError_t launch_attend(const AttendArgs& a, int parts, size_t share, cudaStream_t s) {
-  const size_t smem = Q4Shape<HD>::STAGES * Q4Shape<HD>::STAGE_BYTES + share * sizeof(int32_t);
-  constexpr int MOST = Q4Shape<HD>::STAGES * Q4Shape<HD>::STAGE_BYTES + (int)MAX_SHARE * 4;
+__global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 3) q4_keys_kernel(const AttendArgs a) {
+  __shared__ Query<HD> query;
+  __shared__ int s_max[SPLIT_WARPS];
+  griddep_wait();
+  griddep_launch();
+  Chunk c;
+  if (!c.find(a)) {
+    if (blockIdx.y == 0 && threadIdx.x == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);  // chunk 0 has slots otherwise
+    return;
+  }
+  if (threadIdx.x < 32) lay_out<HD>(query, a.q + c.b * a.ldq + (long long)c.h * HD);
+  __syncthreads();
+  const int mx = keys_pass<HD, SPLIT_WARPS>(a, query, c.slot0, c.n, a.logits + c.slot0);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int m = s_max[0];
+    for (int w = 1; w < SPLIT_WARPS; ++w) m = max(m, s_max[w]);
+    a.chunk_max[(size_t)c.bh * a.chunks + blockIdx.y] = m;
+    if (blockIdx.y == 0) a.arrived[c.bh] = 0;
+  }
+}
+
+// Each chunk's sum of weights: 4 bytes a slot, from the L2 for the most part.
+__global__ void __launch_bounds__(SPLIT_THREADS) q4_sums_kernel(const AttendArgs a) {
+  __shared__ int16_t lut[256];
+  __shared__ unsigned s_red[SPLIT_WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  lut[tid] = d_exp2_lut[tid];
+  griddep_wait();
+  griddep_launch();
+  Chunk c;
+  if (!c.find(a)) return;
+  int mx = INT_MIN;
+  for (int i = lane; i < c.live; i += 32) mx = max(mx, a.chunk_max[(size_t)c.bh * a.chunks + i]);
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if (mx == INT_MIN && tid == 0 && blockIdx.y == 0) nsrl_flag(a.st, NSRL_FLAG_ALL_MASKED);
+  __syncthreads();
+  const unsigned mine = __reduce_add_sync(0xffffffffu, weigh<SPLIT_THREADS>(lut, a.logits + c.slot0, c.n, mx));
+  if (lane == 0) s_red[warp] = mine;
+  __syncthreads();
+  if (tid == 0) {
+    unsigned sum = 0;
+    for (int w = 0; w < SPLIT_WARPS; ++w) sum += s_red[w];
+    a.chunk_sum[(size_t)c.bh * a.chunks + blockIdx.y] = sum;
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_values_kernel(const AttendArgs a) {
+  using S = Q4Shape<HD>;
+  __shared__ __align__(128) uint8_t buffer[SPLIT_WARPS][1024];
+  __shared__ int16_t lut[256];
+  __shared__ uint32_t recip[128];
+  __shared__ long long s_part[SPLIT_WARPS / S::PAIRS][HD];
+  __shared__ unsigned s_arrived;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  lut[tid] = d_exp2_lut[tid];
+  if (tid < 128) recip[tid] = d_recip_lut[tid];
+  griddep_wait();
+  griddep_launch();
+  Chunk c;
+  if (!c.find(a)) return;
+  // every warp adds up the row's chunks for itself
+  int mx = INT_MIN;
+  unsigned long long sum = 0;
+  for (int i = lane; i < c.live; i += 32) {
+    mx = max(mx, a.chunk_max[(size_t)c.bh * a.chunks + i]);
+    sum += a.chunk_sum[(size_t)c.bh * a.chunks + i];
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  const unsigned inv = mx == INT_MIN ? 0u : reciprocal(recip, sum);
+  values_pass<HD, SPLIT_WARPS>(a, c.slot0, c.n, a.logits + c.slot0, lut, mx, inv, buffer[warp],
+                               s_part[warp / S::PAIRS]);
+  __syncthreads();
+  long long total = 0;
+  if (tid < HD) {
+#pragma unroll
+    for (int w = 0; w < SPLIT_WARPS / S::PAIRS; ++w) total += s_part[w][tid];
+  }
+  if (c.live > 1) {
+    // the last chunk to arrive adds up the row's partial contexts
+    long long* const row = a.partial + (size_t)c.bh * a.chunks * HD;
+    if (tid < HD) row[(size_t)blockIdx.y * HD + tid] = total;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_arrived = atomicAdd(&a.arrived[c.bh], 1u);
+    __syncthreads();
+    if (s_arrived != (unsigned)c.live - 1) return;
+    __threadfence();
+    total = 0;
+    if (tid < HD)
+      for (int r = 0; r < c.live; ++r) total += __ldcg(row + (size_t)r * HD + tid);
+  }
+  if (tid < HD) a.ctx[c.b * (long long)(a.c.heads * HD) + (long long)c.h * HD + tid] = sat_i16(rhu64(total, 15));
+}
+
+template <int HD>
+cudaError_t launch_whole(const AttendArgs& a, int parts, size_t share, cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
-  cudaError_t e = allow_smem((const void*)attend_q4_kernel<HD>, MOST, done);
+  cudaError_t e = allow_smem((const void*)attend_q4_kernel<HD>, (int)MAX_SHARE * 4, done);
   if (e == cudaSuccess && parts > 8)
     e = cudaFuncSetAttribute(attend_q4_kernel<HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
@@ -572,35 +661,89 @@ cudaError_t launch_attend(const AttendArgs& a, int parts, size_t share, cudaStre
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.c.batch * a.c.heads * (size_t)parts));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(WHOLE_THREADS);
+  cfg.dynamicSmemBytes = share * sizeof(int32_t);
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = parts > 1 ? 2 : 1;  // a cluster of one would be packed two to an SM while others idle
+  cfg.numAttrs = parts > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, attend_q4_kernel<HD>, a);
+}
+
+template <int HD>
+cudaError_t launch_split(const AttendArgs& a, cudaStream_t s) {
+  const dim3 grid((unsigned)(a.c.batch * a.c.heads), (unsigned)a.chunks), block(SPLIT_THREADS);
+  cudaError_t e = launch_pdl(q4_keys_kernel<HD>, grid, block, 0, s, a);
+  if (e == cudaSuccess) e = launch_pdl(q4_sums_kernel, grid, block, 0, s, a);
+  if (e == cudaSuccess) e = launch_pdl(q4_values_kernel<HD>, grid, block, 0, s, a);
+  return e;
+}
+
+// The form of a call, from what its launch knows (lengths live on the device).
+struct Q4Plan {
+  bool split;
+  int parts;      // WHOLE: CTAs of a row
+  size_t chunks;  // split: of a row
+  size_t logits, chunk_max, chunk_sum, arrived, partial, total;  // scratch offsets and size
+};
+
+Q4Plan plan_of(const nsrl_q4_cache& c) {
+  Q4Plan p{};
+  const size_t bh = c.batch * c.heads, groups = std::max<size_t>(1, c.head_dim / 32);
+  const size_t bytes = bh * c.capacity * (c.head_dim + 8 * groups);
+  p.split = bytes >= SPLIT_BYTES;
+  p.parts = 1;
+  if (!p.split) {
+    while (p.parts < MAX_CLUSTER && ((c.capacity + p.parts - 1) / p.parts > MAX_SHARE ||
+                                     (bh * p.parts < 148 && c.capacity / p.parts >= 512)))
+      p.parts *= 2;
+    return p;
+  }
+  p.chunks = (c.capacity + CHUNK - 1) / CHUNK;
+  auto take = [&](size_t n) {
+    const size_t at = p.total;
+    p.total += (n + 255) & ~size_t(255);
+    return at;
+  };
+  p.logits = take(bh * c.capacity * sizeof(int32_t));
+  p.chunk_max = take(bh * p.chunks * sizeof(int32_t));
+  p.chunk_sum = take(bh * p.chunks * sizeof(unsigned));
+  p.arrived = take(bh * sizeof(unsigned));
+  p.partial = take(bh * p.chunks * c.head_dim * sizeof(long long));
+  return p;
 }
 
 }  // namespace
 
 size_t q4_max_capacity() { return 8 * MAX_SHARE; }
 
+size_t q4_attend_workspace(const nsrl_q4_cache& c) { return plan_of(c).total; }
+
 cudaError_t launch_attend_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache& c, const int32_t* lens, int len_offset,
-                             int16_t* ctx, nsrl_device_status* st, cudaStream_t s) {
+                             int16_t* ctx, void* ws, nsrl_device_status* st, cudaStream_t s) {
   const size_t bh = c.batch * c.heads;
   if (bh == 0) return cudaSuccess;
   if (c.capacity > q4_max_capacity() || bh > 0x7fffffffull / MAX_CLUSTER) return cudaErrorInvalidValue;
-  const AttendArgs a{c, q, (long long)ldq, lens, len_offset, ctx, st};
-  int parts = 1;
-  while (parts < MAX_CLUSTER &&
-         ((c.capacity + parts - 1) / parts > MAX_SHARE || (bh * parts < 148 && c.capacity / parts >= 512)))
-    parts *= 2;
-  const size_t share = ((c.capacity + parts - 1) / parts + SHARE_UNIT - 1) / SHARE_UNIT * SHARE_UNIT;
+  AttendArgs a{c, q, (long long)ldq, lens, len_offset, ctx, st};
+  const Q4Plan p = plan_of(c);
   const double slots = (double)bh * (double)c.capacity;
   ProfScope prof("attention_decode_q4", s, 4.0 * slots * (double)c.head_dim,
                  slots * ((double)c.head_dim + 8.0 * std::max<size_t>(1, c.head_dim / 32) + (c.scores ? 8.0 : 0.0)));
-  const cudaError_t e = c.head_dim == 16   ? launch_attend<16>(a, parts, share, s)
-                        : c.head_dim == 64 ? launch_attend<64>(a, parts, share, s)
-                                           : launch_attend<256>(a, parts, share, s);
+  cudaError_t e;
+  if (p.split) {
+    uint8_t* base = static_cast<uint8_t*>(ws);
+    a.chunks = (int)p.chunks;
+    a.logits = reinterpret_cast<int32_t*>(base + p.logits);
+    a.chunk_max = reinterpret_cast<int32_t*>(base + p.chunk_max);
+    a.chunk_sum = reinterpret_cast<unsigned*>(base + p.chunk_sum);
+    a.arrived = reinterpret_cast<unsigned*>(base + p.arrived);
+    a.partial = reinterpret_cast<long long*>(base + p.partial);
+    e = c.head_dim == 16 ? launch_split<16>(a, s) : c.head_dim == 64 ? launch_split<64>(a, s) : launch_split<256>(a, s);
+  } else {
+    const size_t share = ((c.capacity + p.parts - 1) / p.parts + UNIT - 1) / UNIT * UNIT;
+    e = c.head_dim == 16   ? launch_whole<16>(a, p.parts, share, s)
+        : c.head_dim == 64 ? launch_whole<64>(a, p.parts, share, s)
+                           : launch_whole<256>(a, p.parts, share, s);
+  }
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -286,9 +286,10 @@ cudaError_t launch_q4_evict(const nsrl_q4_cache& c, const int32_t* lens, const i
                             size_t recent, int32_t* scores_out, int32_t* positions_out, int32_t* lens_out, void* ws,
                             nsrl_device_status* st, cudaStream_t s);
 size_t q4_max_capacity();
-// Keys attended: lens[b] + len_offset.
+// Keys attended: lens[b] + len_offset.  ws: q4_attend_workspace bytes, 256-byte aligned.
+size_t q4_attend_workspace(const nsrl_q4_cache& c);
 cudaError_t launch_attend_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache& c, const int32_t* lens, int len_offset,
-                             int16_t* ctx, nsrl_device_status* st, cudaStream_t s);
+                             int16_t* ctx, void* ws, nsrl_device_status* st, cudaStream_t s);
 
 void set_error(const char* fmt, ...);
 bool tma_supported();

@@ -124,6 +124,9 @@ def test_read_saturates_and_refuses(K):
 ATTENDS = [(1, 1, 64, 16, [1]), (2, 3, 64, 64, [31, 33]), (3, 2, 16, 48, [1, 17, 48]), (2, 2, 256, 160, [160, 129]),
            (1, 4, 64, 1024, [1000]), (4, 16, 64, 2048, [2048, 1, 2047, 1025]), (1, 1, 16, 4096, [4095]),
            (40, 8, 64, 272, None), (160, 1, 16, 80, None), (1, 2, 256, 2064, [2050]), (2, 1, 64, 8208, [8193, 64])]
+# large enough for the split form: ragged rows of one chunk, of several, and that end with or just past one
+ATTENDS += [(80, 1, 64, 4112, None), (40, 2, 64, 4112, [1, 2048, 2049, 4096, 4097, 4112, 31, 256] * 5),
+            (130, 2, 16, 4112, None), (20, 2, 256, 2064, None)]
 
 
 @pytest.mark.parametrize("case", ATTENDS)
@@ -179,9 +182,21 @@ def test_attend_long_stream(K):
     cap = 100000
     cache, kv, vv = filled(K, rng, 1, 1, 64, cap, True, 8, 4096)
     q = gaussian(rng, (1, 1, 64), 8)
-    for n in (cap, 50001):
+    for n in (cap, 50001):  # eight CTAs of a cluster
         ctx, scores = P.attend(q, kv, vv, [n], host(cache.scores))
         assert np.array_equal(host(cache.attend(dev(q.reshape(1, 64)), i32([n]))), ctx)
+        assert np.array_equal(host(cache.scores), scores)
+
+
+def test_attend_long_streams_split(K):
+    """Four streams of 100,000 slots: chunks of several CTAs, added up by the last to arrive."""
+    rng = np.random.default_rng(16)
+    cap = 100000
+    cache, kv, vv = filled(K, rng, 1, 4, 64, cap, True, 8, 4096)
+    q = gaussian(rng, (1, 4, 64), 8)
+    for n in (cap, 65537, 3):
+        ctx, scores = P.attend(q, kv, vv, [n], host(cache.scores))
+        assert np.array_equal(host(cache.attend(dev(q.reshape(1, 256)), i32([n]))), ctx)
         assert np.array_equal(host(cache.scores), scores)
 
 
@@ -195,38 +210,42 @@ def test_scores_saturate(K):
     assert np.array_equal(host(cache.scores), scores)
 
 
-@pytest.mark.parametrize("lens", [[0, 5], [5, 17], [-3, 5]])
-def test_attend_rejects_bad_lengths(K, lens):
-    rng = np.random.default_rng(7)
-    cache, _, _ = filled(K, rng, 2, 2, 64, 16)
-    assert cache.attend(dev(gaussian(rng, (2, 128), 32)), i32(lens)) is None
+@pytest.mark.parametrize("cap", [16, 81920])  # one launch, and the split form
+@pytest.mark.parametrize("lens", [[0, 5], [5, -1], [-3, 5]])
+def test_attend_rejects_bad_lengths(K, lens, cap):
+    cache = K.Q4Cache(2, 2, 64, cap)
+    q = torch.ones((2, 128), dtype=torch.int16, device="cuda")
+    assert cache.attend(q, i32([5, cap])) is not None
+    assert cache.attend(q, i32([cap + 1 if n < 0 and n != -3 else n for n in lens])) is None
 
 
-@pytest.mark.parametrize("hd", [64, 256])
-def test_attend_rejects_logits_outside_i32(K, hd):
+@pytest.mark.parametrize("hd,cap", [(64, 16), (256, 16), (64, 262144), (256, 262144)])
+def test_attend_rejects_logits_outside_i32(K, hd, cap):
     """q = k = 32767: (hd 2^30) >> log4(hd) is 2^33 (64 dims) and 2^34 (256)."""
-    cache = K.Q4Cache(1, 1, hd, 16)
+    cache = K.Q4Cache(1, 1, hd, cap)
     x = torch.full((16, hd), 32767, dtype=torch.int16, device="cuda")
     assert cache.append(x, x, i32([0])) is True
     assert cache.attend(x[:1], i32([16])) is None
 
 
-def test_masked_logits(K):
+@pytest.mark.parametrize("cap", [16, 262144])
+def test_masked_logits(K, cap):
     """A logit of exactly -2^31 is the reference's MASKED_LOGIT: no weight; all of them: a rejection.
     Values 32768 (zero 32767, scale 1, code 1) times q = -32768 on 16 of 64 dims: -2^34 >> 3."""
-    cache = K.Q4Cache(1, 1, 64, 16)
+    cache = K.Q4Cache(2, 1, 64, cap)  # the larger takes the split form
     cache.k_scales.fill_(1 | (32767 << 16))
     cache.k_codes.fill_(0x11)
     cache.v_scales[..., :] = 1 | (100 << 16)
-    q = torch.zeros((1, 64), dtype=torch.int16, device="cuda")
+    q = torch.zeros((2, 64), dtype=torch.int16, device="cuda")
     q[:, :16] = -32768
-    assert cache.attend(q, i32([16])) is None
-    cache.k_codes[0, 0, 3] = 0  # slot 3: 32767 -> -32768 * 32767 * 16 >> 3, above the others
-    cache.v_scales[0, 0, 3] = 1 | (7000 << 16)
-    got = cache.attend(q, i32([16]))
+    assert cache.attend(q, i32([16, 16])) is None
+    cache.k_codes[:, 0, 3] = 0  # slot 3: 32767 -> -32768 * 32767 * 16 >> 3, above the others
+    cache.v_scales[:, 0, 3] = 1 | (7000 << 16)
+    got = cache.attend(q, i32([16, 16]))
     want = O.attention_row(np.zeros(64, np.int16), np.zeros((1, 64), np.int16), np.full((1, 64), 7000, np.int16), 64, 64)
-    assert np.array_equal(host(got)[0], want[0])
-    assert host(cache.scores)[0, 0].tolist() == [0] * 3 + [int(want[2][0])] + [0] * 12
+    for b in range(2):
+        assert np.array_equal(host(got)[b], want[0])
+        assert host(cache.scores)[b, 0, :16].tolist() == [0] * 3 + [int(want[2][0])] + [0] * 12
 
 
 # ---------------------------------------------------------------- eviction ---

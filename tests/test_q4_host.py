@@ -106,7 +106,8 @@ def test_cache_refusals(lib, bad):
     c = q4(**bad)
     assert lib.nsrl_q4_cache_append(c, P16, P16, 256, 1, P16, None, None, P16, None) == 1
     assert lib.nsrl_q4_cache_read(c, None, 1, P16, P16, P16, None) == 1
-    assert lib.nsrl_attention_decode_q4(P16, 256, c, P16, P16, P16, None) == 1
+    assert lib.nsrl_attention_decode_q4(P16, 256, c, P16, P16, None, 0, P16, None) == 1
+    assert lib.nsrl_attention_decode_q4_workspace_size(c) == 0 and lib.nsrl_decode_block_q4_workspace_size(c) == 0
     assert lib.nsrl_q4_cache_evict(c, P16, P16, 8, 0, 0, P16, P16, P16, P16, 1 << 40, P16, None) == 1
     assert lib.nsrl_q4_cache_evict_workspace_size(c, 8) == 0
     assert b"invalid shape" in lib.nsrl_last_error()
@@ -129,12 +130,17 @@ def test_append_and_read_refusals(lib):
 
 def test_attend_refusals(lib):
     f = lib.nsrl_attention_decode_q4
-    assert f(P16, 255, q4(), P16, P16, P16, None) == 1
-    for i in (0, 3, 4, 5):
-        args = [P16, 256, q4(), P16, P16, P16, None]
+    assert f(P16, 255, q4(), P16, P16, None, 0, P16, None) == 1
+    for i in (0, 3, 4, 7):
+        args = [P16, 256, q4(), P16, P16, None, 0, P16, None]
         args[i] = None
         assert f(*args) == 1
-    assert f(None, 256, q4(batch=0), None, None, None, None) == 0
+    assert f(None, 256, q4(batch=0), None, None, None, 0, None, None) == 0
+    big = q4(batch=64, capacity=8192)  # takes a workspace
+    ws = lib.nsrl_attention_decode_q4_workspace_size(big)
+    assert ws >= 4 * 64 * 4 * 8192
+    for w, n in ((None, ws), (P16, ws), (C.c_void_p(256), ws - 1)):
+        assert f(P16, 256, big, P16, P16, w, n, P16, None) == 1
 
 
 def test_evict_refusals(lib):
@@ -173,12 +179,13 @@ def test_decode_block_refusals(lib):
     from nsrl_b200.core import LinearParamsC as LP
     f = lib.nsrl_prenorm_attention_decode_block_q4
     lin = LP(16, None, 16, 256, 256)
-    ws = lib.nsrl_decode_block_q4_workspace_size(2, 256, 4)
+    ws = lib.nsrl_decode_block_q4_workspace_size(q4())
+    p256 = C.c_void_p(256)
 
-    def call(x=P16, batch=2, d=256, heads=4, gamma=P16, lp=lin, cache=None, lens=P16, y=P16, w=P16, wb=ws, st=P16):
+    def call(x=P16, batch=2, d=256, heads=4, gamma=P16, lp=lin, cache=None, lens=P16, y=P16, w=p256, wb=ws, st=P16):
         return f(x, batch, d, heads, gamma, 1, *[C.byref(lp)] * 4, None, cache or q4(), lens, None, y, w, wb, st, None)
 
     for bad in (dict(batch=3), dict(heads=2), dict(lp=LP(16, None, 16, 256, 128)), dict(cache=q4(head_dim=16)),
-                dict(x=None), dict(gamma=None), dict(lens=None), dict(y=None), dict(w=None), dict(wb=ws - 1),
+                dict(x=None), dict(gamma=None), dict(lens=None), dict(y=None), dict(w=None), dict(w=P16), dict(wb=ws - 1),
                 dict(st=None), dict(d=512)):
         assert call(**bad) == 1, bad
