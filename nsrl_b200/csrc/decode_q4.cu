@@ -247,44 +247,59 @@ __device__ __forceinline__ void dots16(const Query<HD>& query, const KeyRow<HD> 
 }
 
 // Logits of n slots from slot0; returns this warp's maximum (INT_MIN: none
-// counts; MASKED_LOGIT is INT_MIN and never raises it).  A step takes R units,
-// the next step's rows under way where registers allow.
-template <int HD, int WARPS>
+// counts; MASKED_LOGIT is INT_MIN and never raises it).  A step takes two whole
+// units with the next step's rows under way (one unit and none ahead at 256
+// dims, whose rows fill the registers); what is left over goes unit by unit.
+// `ready` is called once, after the first loads and before the query is read.
+template <int HD, int WARPS, typename Ready>
 __device__ __forceinline__ int keys_pass(const AttendArgs& a, const Query<HD>& query, size_t slot0, int n,
-                                         int32_t* logits) {
+                                         int32_t* logits, Ready ready) {
   using S = Q4Shape<HD>;
-  constexpr int R = HD == 256 ? 1 : 2, APART = UNIT * WARPS;
-  constexpr bool AHEAD = HD != 256;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int mx = INT_MIN;
   bool bad = false;
-  KeyRow<HD> row[R], next[AHEAD ? R : 1];
-  int j = UNIT * warp + lane;
-  if constexpr (AHEAD) {
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (j + r * APART < n) next[r].load(a.c, slot0 + j + r * APART);
+  auto put = [&](int j, long long v) {
+    const long long lg = v >> (S::SHIFT + 4);
+    bad = bad || lg != (long long)(int)lg;
+    logits[j] = (int)lg;
+    mx = max(mx, (int)lg);
+  };
+  const int whole = n / UNIT;
+  int u = warp;
+  if constexpr (HD != 256) {
+    KeyRow<HD> row[2], next[2];
+    bool two = u + WARPS < whole;
+    if (two) {
+      next[0].load(a.c, slot0 + u * UNIT + lane);
+      next[1].load(a.c, slot0 + (u + WARPS) * UNIT + lane);
+    }
+    ready();
+    while (two) {
+      row[0] = next[0];
+      row[1] = next[1];
+      const int at = u * UNIT + lane;
+      u += 2 * WARPS;
+      two = u + WARPS < whole;
+      if (two) {
+        next[0].load(a.c, slot0 + u * UNIT + lane);
+        next[1].load(a.c, slot0 + (u + WARPS) * UNIT + lane);
+      }
+      long long v[2];
+      dots16<HD, 2>(query, row, v);
+      put(at, v[0]);
+      put(at + WARPS * UNIT, v[1]);
+    }
+  } else {
+    ready();
   }
-  for (; j < n; j += R * APART) {
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) row[r] = next[r];
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (j + (R + r) * APART < n) next[r].load(a.c, slot0 + j + (R + r) * APART);
-    } else {
-      row[0].load(a.c, slot0 + j);
-    }
-    long long v[R];
-    dots16<HD, R>(query, row, v);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (j + r * APART >= n) break;
-      const long long lg = v[r] >> (S::SHIFT + 4);
-      bad = bad || lg != (long long)(int)lg;
-      logits[j + r * APART] = (int)lg;
-      mx = max(mx, (int)lg);
-    }
+  for (; u * UNIT < n; u += WARPS) {
+    const int j = u * UNIT + lane;
+    if (j >= n) continue;
+    KeyRow<HD> row[1];
+    row[0].load(a.c, slot0 + j);
+    long long v[1];
+    dots16<HD, 1>(query, row, v);
+    put(j, v[0]);
   }
   if (bad) nsrl_flag(a.st, NSRL_FLAG_LOGIT_RANGE);
   return __reduce_max_sync(0xffffffffu, mx);
@@ -304,29 +319,42 @@ struct ValueUnit {
   uint4 code[2];  // HD 16: the first 8 bytes
   uint2 scale;
   int logit, score;
+};
 
-  // left: slots from the unit's first one to the end
-  __device__ __forceinline__ void load(const nsrl_q4_cache& c, size_t slot, int pair, int own, int left,
-                                       const int32_t* logits, const int32_t* scores) {
+// This lane's places in a warp's first unit; a unit further on they move by constants.
+template <int HD>
+struct ValuePlaces {
+  using S = Q4Shape<HD>;
+  const uint8_t* code;
+  const uint32_t* scale;
+  const int32_t* logit;
+  int32_t* score;  // NULL: no scores, or another warp's to keep
+  int own;
+
+  // WHOLE: every slot of the unit is there; otherwise `left` of them are
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(ValueUnit<HD>& u, int unit, int left) const {
     const int lane = threadIdx.x & 31;
     // rows past the end are inside the capacity up to the next multiple of 16 slots
     const int last = (left + 15) & ~15;
+    const uint8_t* c = code + (size_t)(unsigned)unit * (UNIT * HD / 2);
     if constexpr (HD == 16) {
-      const uint2 x = lane < last ? __ldcs(reinterpret_cast<const uint2*>(c.v_codes) + slot + lane) : make_uint2(0, 0);
-      code[0].x = x.x, code[0].y = x.y;
-      scale = make_uint2(own < left ? __ldcs(c.v_scales + slot + own) : 0u, 0u);
+      const uint2 x = WHOLE || lane < last ? __ldcs(reinterpret_cast<const uint2*>(c)) : make_uint2(0, 0);
+      u.code[0].x = x.x, u.code[0].y = x.y;
     } else {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 16 * e + (lane >> 1);
-        code[e] = r < last ? __ldcs(reinterpret_cast<const uint4*>(c.v_codes + (slot + r) * (HD / 2) + 32 * pair) + (lane & 1))
-                           : make_uint4(0, 0, 0, 0);
-      }
-      scale = own < left ? __ldcs(reinterpret_cast<const uint2*>(c.v_scales + (slot + own) * Q4Shape<HD>::G) + pair)
-                         : make_uint2(0, 0);
+      for (int e = 0; e < 2; ++e)
+        u.code[e] = WHOLE || 16 * e + (lane >> 1) < last ? __ldcs(reinterpret_cast<const uint4*>(c + e * 16 * (HD / 2)))
+                                                         : make_uint4(0, 0, 0, 0);
     }
-    logit = own < left ? logits[own] : INT_MIN;
-    score = scores && own < left ? scores[own] : 0;
+    const bool mine = WHOLE || own < left;
+    const uint32_t* s = scale + (size_t)(unsigned)unit * (UNIT * S::G);
+    if constexpr (HD == 16)
+      u.scale = make_uint2(mine ? __ldcs(s) : 0u, 0u);
+    else
+      u.scale = mine ? __ldcs(reinterpret_cast<const uint2*>(s)) : make_uint2(0, 0);
+    u.logit = mine ? logit[unit * UNIT] : INT_MIN;
+    u.score = score && mine ? score[unit * UNIT] : 0;
   }
 };
 
@@ -339,7 +367,7 @@ __device__ __forceinline__ void values_pass(const AttendArgs& a, size_t slot0, i
   constexpr int MMAS = HD == 16 ? 1 : 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int pair = warp % S::PAIRS;
-  const int step = UNIT * (WARPS / S::PAIRS);
+  constexpr int STEP = WARPS / S::PAIRS;  // units from one of this warp's to its next
   int acc[MMAS][4];
 #pragma unroll
   for (int i = 0; i < MMAS; ++i)
@@ -350,21 +378,21 @@ __device__ __forceinline__ void values_pass(const AttendArgs& a, size_t slot0, i
   const int own = 16 * (g >> 2) + (HD == 16 ? 4 * t + (g & 3) : 8 * (t >> 1) + 2 * (g & 3) + (t & 1));
   const int from = 4 * t + (g & 3);  // the lane with plane g & 3 of the slots of k = 4 t; 16 further, of 16 + 4 t
   const uint32_t byte2 = (uint32_t)(g & 3) | ((uint32_t)((g & 3) + 4) << 4);  // byte g & 3 of two words
-  int32_t* const scores = a.c.scores && pair == 0 ? a.c.scores + slot0 : nullptr;
+  ValuePlaces<HD> at;
+  at.own = own;
+  at.code = HD == 16 ? a.c.v_codes + (slot0 + lane) * (HD / 2)
+                     : a.c.v_codes + (slot0 + (lane >> 1)) * (HD / 2) + 32 * pair + 16 * (lane & 1);
+  at.scale = a.c.v_scales + (slot0 + own) * S::G + (HD == 16 ? 0 : 2 * pair);
+  at.logit = logits + own;
+  at.score = a.c.scores && pair == 0 ? a.c.scores + slot0 + own : nullptr;
   // Rows of 32 bytes in the warp's buffer, the halves of rows 4 .. 7 of eight
   // swapped so that the matrix loads' eight rows meet no bank twice.
   const uint32_t store_at = smem_u32(buffer) + 32 * (lane >> 1) + 16 * ((lane & 1) ^ ((lane >> 3) & 1));
   const uint32_t load_at = smem_u32(buffer) + 32 * lane + 16 * ((lane >> 2) & 1);
-  ValueUnit<HD> unit, next;
-  int r = UNIT * (warp / S::PAIRS);
-  if (r < n) next.load(a.c, slot0 + r, pair, own, n - r, logits + r, scores ? scores + r : nullptr);
-  for (; r < n; r += step) {
-    unit = next;
-    const int ahead = r + step;
-    if (ahead < n) next.load(a.c, slot0 + ahead, pair, own, n - ahead, logits + ahead, scores ? scores + ahead : nullptr);
+  auto add = [&](const ValueUnit<HD>& unit, int32_t* score) {  // score: NULL, or this lane's slot's
     const int p =
         unit.logit == INT_MIN ? 0 : (int)min((weight(lut, unit.logit, mx) * inv + 32768u) >> 16, 32767u);
-    if (scores && r + own < n) scores[r + own] = add_sat(unit.score, p);
+    if (score) *score = add_sat(unit.score, p);
     uint32_t w[8];
     if constexpr (HD == 16) {
       *reinterpret_cast<uint2*>(buffer + 8 * lane) = make_uint2(unit.code[0].x, unit.code[0].y);
@@ -412,6 +440,22 @@ __device__ __forceinline__ void values_pass(const AttendArgs& a, size_t slot0, i
       const uint32_t frag[4] = {x, x & HIGH, y, y & HIGH};
       mma_u8u8(acc[i], frag, bf);
     }
+  };
+  const int whole = n / UNIT;
+  int u = warp / S::PAIRS;
+  ValueUnit<HD> unit, next;
+  if (u < whole) at.template load<true>(next, u, UNIT);
+  while (u < whole) {
+    unit = next;
+    const int here = u;
+    u += STEP;
+    if (u < whole) at.template load<true>(next, u, UNIT);
+    add(unit, at.score ? at.score + here * UNIT : nullptr);
+  }
+  if (u == whole && n % UNIT != 0) {
+    const int left = n % UNIT;
+    at.template load<false>(unit, u, left);
+    add(unit, at.score && own < left ? at.score + u * UNIT : nullptr);
   }
   // Columns 2 t and 2 t + 1 are planes 2 (t & 1) and 2 (t & 1) + 1 of group t >> 1
   // of the pair.  s32 is enough: 255 * 255 a slot over at most 8,192 slots a warp.
@@ -473,12 +517,12 @@ __global__ void __launch_bounds__(WHOLE_THREADS, HD == 256 ? 1 : 2) attend_q4_ke
   const long long first = (long long)part * share;
   const int n = (int)max(0ll, min((long long)share, len - first));
   const size_t slot0 = (size_t)bh * a.c.capacity + (size_t)first;
-  if (parts > 1)
-    cluster.sync();  // every CTA has started: its shared memory may be written
-  else
-    __syncthreads();
-
-  int mx = keys_pass<HD, WHOLE_WARPS>(a, query, slot0, n, logits);
+  int mx = keys_pass<HD, WHOLE_WARPS>(a, query, slot0, n, logits, [&] {
+    if (parts > 1)
+      cluster.sync();  // every CTA has started: its shared memory may be written
+    else
+      __syncthreads();
+  });
   if (lane == 0) s_redi[warp] = mx;
   __syncthreads();
 #pragma unroll
@@ -552,13 +596,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 3) q4_keys_kern
   griddep_wait();
   griddep_launch();
   Chunk c;
-  if (!c.find(a)) {
+  const bool there = c.find(a);
+  if (threadIdx.x < 32) lay_out<HD>(query, a.q + c.b * a.ldq + (long long)c.h * HD);
+  if (!there) {
     if (blockIdx.y == 0 && threadIdx.x == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);  // chunk 0 has slots otherwise
     return;
   }
-  if (threadIdx.x < 32) lay_out<HD>(query, a.q + c.b * a.ldq + (long long)c.h * HD);
-  __syncthreads();
-  const int mx = keys_pass<HD, SPLIT_WARPS>(a, query, c.slot0, c.n, a.logits + c.slot0);
+  const int mx = keys_pass<HD, SPLIT_WARPS>(a, query, c.slot0, c.n, a.logits + c.slot0, [] { __syncthreads(); });
   if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
   __syncthreads();
   if (threadIdx.x == 0) {
