@@ -17,6 +17,7 @@
 //           sum, VALUES each chunk's context; the last chunk of a row to arrive
 //           adds them up (integers: in any order the same).  No CTA waits for
 //           another, and chunks spread evenly over the SMs.
+// plan_of() chooses, by sizes alone.
 //
 // Bound by memory (80 bytes a slot of 64 dims, 88 with scores) while an SM
 // spends less than about 3.5 cycles on a slot, that is some 14 instructions of
@@ -49,7 +50,8 @@ constexpr int MAX_CLUSTER = 16;
 constexpr int UNIT = 32;             // slots of a warp's step
 constexpr size_t MAX_SHARE = 32768;  // logits of a CTA: 128 KB
 constexpr int CHUNK = 2048;          // slots of a CTA of the split form
-constexpr size_t SPLIT_BYTES = 24u << 20;  // cache bytes from which a call takes the split form
+constexpr int FEW_SLOTS = 2048;      // up to which a CTA of the one-launch form has 8 warps, 16 above
+constexpr size_t SPLIT_SLOTS = MAX_CLUSTER * FEW_SLOTS;  // capacity from which few rows take the split form
 
 template <int HD>
 struct Q4Shape {
@@ -321,77 +323,88 @@ struct ValueUnit {
   int logit, score;
 };
 
-// This lane's places in a warp's first unit; a unit further on they move by constants.
-template <int HD>
+// This lane's places in a row's (or chunk's) first unit; a unit further on they
+// move by constants.  FAR: the logits are in global memory and come with the
+// rows; otherwise they are read from shared memory when they are due.
+template <int HD, bool FAR>
 struct ValuePlaces {
   using S = Q4Shape<HD>;
   const uint8_t* code;
   const uint32_t* scale;
   const int32_t* logit;
   int32_t* score;  // NULL: no scores, or another warp's to keep
-  int own;
+  int own, pair;
 
-  // WHOLE: every slot of the unit is there; otherwise `left` of them are
-  template <bool WHOLE>
+  __device__ __forceinline__ ValuePlaces(const AttendArgs& a, size_t slot0, const int32_t* logits) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    pair = warp % S::PAIRS;
+    // The quad's slots are those of k = 4 (g & 3) + 16 (g >> 2) and the three after it.
+    own = 16 * (g >> 2) + (HD == 16 ? 4 * t + (g & 3) : 8 * (t >> 1) + 2 * (g & 3) + (t & 1));
+    code = HD == 16 ? a.c.v_codes + (slot0 + lane) * (HD / 2)
+                    : a.c.v_codes + (slot0 + (lane >> 1)) * (HD / 2) + 32 * pair + 16 * (lane & 1);
+    scale = a.c.v_scales + (slot0 + own) * S::G + (HD == 16 ? 0 : 2 * pair);
+    logit = logits + own;
+    score = a.c.scores && pair == 0 ? a.c.scores + slot0 + own : nullptr;
+  }
+
+  // ALL: every slot of the unit is there; otherwise `left` of them are
+  template <bool ALL>
   __device__ __forceinline__ void load(ValueUnit<HD>& u, int unit, int left) const {
     const int lane = threadIdx.x & 31;
     // rows past the end are inside the capacity up to the next multiple of 16 slots
     const int last = (left + 15) & ~15;
     const uint8_t* c = code + (size_t)(unsigned)unit * (UNIT * HD / 2);
     if constexpr (HD == 16) {
-      const uint2 x = WHOLE || lane < last ? __ldcs(reinterpret_cast<const uint2*>(c)) : make_uint2(0, 0);
+      const uint2 x = ALL || lane < last ? __ldcs(reinterpret_cast<const uint2*>(c)) : make_uint2(0, 0);
       u.code[0].x = x.x, u.code[0].y = x.y;
     } else {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        u.code[e] = WHOLE || 16 * e + (lane >> 1) < last ? __ldcs(reinterpret_cast<const uint4*>(c + e * 16 * (HD / 2)))
+        u.code[e] = ALL || 16 * e + (lane >> 1) < last ? __ldcs(reinterpret_cast<const uint4*>(c + e * 16 * (HD / 2)))
                                                          : make_uint4(0, 0, 0, 0);
     }
-    const bool mine = WHOLE || own < left;
+    const bool mine = ALL || own < left;
     const uint32_t* s = scale + (size_t)(unsigned)unit * (UNIT * S::G);
     if constexpr (HD == 16)
       u.scale = make_uint2(mine ? __ldcs(s) : 0u, 0u);
     else
       u.scale = mine ? __ldcs(reinterpret_cast<const uint2*>(s)) : make_uint2(0, 0);
-    u.logit = mine ? logit[unit * UNIT] : INT_MIN;
+    if (FAR) u.logit = mine ? logit[unit * UNIT] : INT_MIN;
     u.score = score && mine ? score[unit * UNIT] : 0;
   }
 };
 
-// Context of n slots from slot0 into part[HD] (this warp's row; only the pair's dims are written).
-template <int HD, int WARPS>
-__device__ __forceinline__ void values_pass(const AttendArgs& a, size_t slot0, int n, const int32_t* logits,
+// The first unit of this warp, asked for ahead of values_pass.
+template <int HD, int WARPS, bool FAR>
+__device__ __forceinline__ void first_values(const ValuePlaces<HD, FAR>& at, int n, ValueUnit<HD>& next) {
+  const int u = (int)(threadIdx.x >> 5) / Q4Shape<HD>::PAIRS;
+  if ((u + 1) * UNIT <= n) at.template load<true>(next, u, UNIT);
+}
+
+// Context of n slots into part[HD] (this warp's row; only the pair's dims are written).
+template <int HD, int WARPS, bool FAR>
+__device__ __forceinline__ void values_pass(const ValuePlaces<HD, FAR>& at, ValueUnit<HD> next, int n,
                                             const int16_t* lut, int mx, unsigned inv, uint8_t* buffer,
                                             long long* part) {
   using S = Q4Shape<HD>;
   constexpr int MMAS = HD == 16 ? 1 : 4;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int pair = warp % S::PAIRS;
   constexpr int STEP = WARPS / S::PAIRS;  // units from one of this warp's to its next
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int pair = at.pair, own = at.own;
   int acc[MMAS][4];
 #pragma unroll
   for (int i = 0; i < MMAS; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = 0;
   long long zero_part[2] = {0, 0};  // sum of p zero over this lane's slots, per group of the pair
-  // The quad's slots are those of k = 4 (g & 3) + 16 (g >> 2) and the three after it.
-  const int own = 16 * (g >> 2) + (HD == 16 ? 4 * t + (g & 3) : 8 * (t >> 1) + 2 * (g & 3) + (t & 1));
   const int from = 4 * t + (g & 3);  // the lane with plane g & 3 of the slots of k = 4 t; 16 further, of 16 + 4 t
   const uint32_t byte2 = (uint32_t)(g & 3) | ((uint32_t)((g & 3) + 4) << 4);  // byte g & 3 of two words
-  ValuePlaces<HD> at;
-  at.own = own;
-  at.code = HD == 16 ? a.c.v_codes + (slot0 + lane) * (HD / 2)
-                     : a.c.v_codes + (slot0 + (lane >> 1)) * (HD / 2) + 32 * pair + 16 * (lane & 1);
-  at.scale = a.c.v_scales + (slot0 + own) * S::G + (HD == 16 ? 0 : 2 * pair);
-  at.logit = logits + own;
-  at.score = a.c.scores && pair == 0 ? a.c.scores + slot0 + own : nullptr;
   // Rows of 32 bytes in the warp's buffer, the halves of rows 4 .. 7 of eight
   // swapped so that the matrix loads' eight rows meet no bank twice.
   const uint32_t store_at = smem_u32(buffer) + 32 * (lane >> 1) + 16 * ((lane & 1) ^ ((lane >> 3) & 1));
   const uint32_t load_at = smem_u32(buffer) + 32 * lane + 16 * ((lane >> 2) & 1);
-  auto add = [&](const ValueUnit<HD>& unit, int32_t* score) {  // score: NULL, or this lane's slot's
-    const int p =
-        unit.logit == INT_MIN ? 0 : (int)min((weight(lut, unit.logit, mx) * inv + 32768u) >> 16, 32767u);
+  auto add = [&](const ValueUnit<HD>& unit, int logit, int32_t* score) {  // score: NULL, or this lane's slot's
+    const int p = logit == INT_MIN ? 0 : (int)min((weight(lut, logit, mx) * inv + 32768u) >> 16, 32767u);
     if (score) *score = add_sat(unit.score, p);
     uint32_t w[8];
     if constexpr (HD == 16) {
@@ -443,19 +456,19 @@ __device__ __forceinline__ void values_pass(const AttendArgs& a, size_t slot0, i
   };
   const int whole = n / UNIT;
   int u = warp / S::PAIRS;
-  ValueUnit<HD> unit, next;
-  if (u < whole) at.template load<true>(next, u, UNIT);
+  ValueUnit<HD> unit;
   while (u < whole) {
     unit = next;
-    const int here = u;
+    const int here = u * UNIT;
     u += STEP;
     if (u < whole) at.template load<true>(next, u, UNIT);
-    add(unit, at.score ? at.score + here * UNIT : nullptr);
+    add(unit, FAR ? unit.logit : at.logit[here], at.score ? at.score + here : nullptr);
   }
   if (u == whole && n % UNIT != 0) {
     const int left = n % UNIT;
     at.template load<false>(unit, u, left);
-    add(unit, at.score && own < left ? at.score + u * UNIT : nullptr);
+    const bool mine = own < left;
+    add(unit, !mine ? INT_MIN : FAR ? unit.logit : at.logit[u * UNIT], mine && at.score ? at.score + u * UNIT : nullptr);
   }
   // Columns 2 t and 2 t + 1 are planes 2 (t & 1) and 2 (t & 1) + 1 of group t >> 1
   // of the pair.  s32 is enough: 255 * 255 a slot over at most 8,192 slots a warp.
@@ -477,8 +490,6 @@ __device__ __forceinline__ void values_pass(const AttendArgs& a, size_t slot0, i
 }
 
 // --------------------------------------------------------------- one launch
-constexpr int WHOLE_WARPS = 16, WHOLE_THREADS = 32 * WHOLE_WARPS;
-
 // Gives `value` to entry `part` of every CTA of the cluster; all of them are
 // here once the cluster has synchronised.
 template <typename T>
@@ -487,18 +498,19 @@ __device__ __forceinline__ void share_out(const cg::cluster_group& cluster, T* v
   cluster.sync();
 }
 
-template <int HD>
-__global__ void __launch_bounds__(WHOLE_THREADS, HD == 256 ? 1 : 2) attend_q4_kernel(const AttendArgs a) {
+template <int HD, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARPS) attend_q4_kernel(const AttendArgs a) {
   using S = Q4Shape<HD>;
+  constexpr int THREADS = 32 * WARPS;
   extern __shared__ __align__(16) int32_t logits[];
   __shared__ Query<HD> query;
-  __shared__ __align__(128) uint8_t buffer[WHOLE_WARPS][1024];
+  __shared__ __align__(128) uint8_t buffer[WARPS][1024];
   __shared__ int16_t lut[256];
   __shared__ uint32_t recip[128];
-  __shared__ int s_max[MAX_CLUSTER], s_redi[WHOLE_WARPS];
-  __shared__ unsigned s_red[WHOLE_WARPS];
+  __shared__ int s_max[MAX_CLUSTER], s_redi[WARPS];
+  __shared__ unsigned s_red[WARPS];
   __shared__ unsigned long long s_sum[MAX_CLUSTER];
-  __shared__ long long s_part[WHOLE_WARPS / S::PAIRS][HD], s_ctx[HD];
+  __shared__ long long s_part[WARPS / S::PAIRS][HD], s_ctx[HD];
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -517,40 +529,43 @@ __global__ void __launch_bounds__(WHOLE_THREADS, HD == 256 ? 1 : 2) attend_q4_ke
   const long long first = (long long)part * share;
   const int n = (int)max(0ll, min((long long)share, len - first));
   const size_t slot0 = (size_t)bh * a.c.capacity + (size_t)first;
-  int mx = keys_pass<HD, WHOLE_WARPS>(a, query, slot0, n, logits, [&] {
+  int mx = keys_pass<HD, WARPS>(a, query, slot0, n, logits, [&] {
     if (parts > 1)
       cluster.sync();  // every CTA has started: its shared memory may be written
     else
       __syncthreads();
   });
+  const ValuePlaces<HD, false> at(a, slot0, logits);
+  ValueUnit<HD> next;
+  first_values<HD, WARPS>(at, n, next);  // under way while the softmax is worked out
   if (lane == 0) s_redi[warp] = mx;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < WHOLE_WARPS; ++w) mx = max(mx, s_redi[w]);
+  for (int w = 0; w < WARPS; ++w) mx = max(mx, s_redi[w]);
   if (parts > 1) {
     share_out(cluster, s_max, mx, part, parts);
     for (int r = 0; r < parts; ++r) mx = max(mx, s_max[r]);
   }
   if (mx == INT_MIN && tid == 0 && part == 0) nsrl_flag(a.st, NSRL_FLAG_ALL_MASKED);
   // Only the sum: the value pass weighs each slot again.  A CTA's sum is at most 2^15 * MAX_SHARE = 2^30.
-  const unsigned mine = __reduce_add_sync(0xffffffffu, weigh<WHOLE_THREADS>(lut, logits, n, mx));
+  const unsigned mine = __reduce_add_sync(0xffffffffu, weigh<THREADS>(lut, logits, n, mx));
   if (lane == 0) s_red[warp] = mine;
   __syncthreads();
   unsigned long long sum = 0;
 #pragma unroll
-  for (int w = 0; w < WHOLE_WARPS; ++w) sum += s_red[w];
+  for (int w = 0; w < WARPS; ++w) sum += s_red[w];
   if (parts > 1) {
     share_out(cluster, s_sum, sum, part, parts);
     sum = 0;
     for (int r = 0; r < parts; ++r) sum += s_sum[r];
   }
   const unsigned inv = mx == INT_MIN ? 0u : reciprocal(recip, sum);
-  values_pass<HD, WHOLE_WARPS>(a, slot0, n, logits, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
+  values_pass<HD, WARPS>(at, next, n, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
   __syncthreads();
   long long total = 0;
   if (tid < HD) {
 #pragma unroll
-    for (int w = 0; w < WHOLE_WARPS / S::PAIRS; ++w) total += s_part[w][tid];
+    for (int w = 0; w < WARPS / S::PAIRS; ++w) total += s_part[w][tid];
   }
   if (parts > 1) {
     if (tid < HD) s_ctx[tid] = total;
@@ -590,7 +605,7 @@ struct Chunk {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 3) q4_keys_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_keys_kernel(const AttendArgs a) {
   __shared__ Query<HD> query;
   __shared__ int s_max[SPLIT_WARPS];
   griddep_wait();
@@ -653,6 +668,9 @@ __global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_values_ke
   griddep_launch();
   Chunk c;
   if (!c.find(a)) return;
+  const ValuePlaces<HD, true> at(a, c.slot0, a.logits + c.slot0);
+  ValueUnit<HD> next;
+  first_values<HD, SPLIT_WARPS>(at, c.n, next);
   // every warp adds up the row's chunks for itself
   int mx = INT_MIN;
   unsigned long long sum = 0;
@@ -665,8 +683,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_values_ke
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   __syncthreads();
   const unsigned inv = mx == INT_MIN ? 0u : reciprocal(recip, sum);
-  values_pass<HD, SPLIT_WARPS>(a, c.slot0, c.n, a.logits + c.slot0, lut, mx, inv, buffer[warp],
-                               s_part[warp / S::PAIRS]);
+  values_pass<HD, SPLIT_WARPS>(at, next, c.n, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
   __syncthreads();
   long long total = 0;
   if (tid < HD) {
@@ -690,12 +707,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_values_ke
   if (tid < HD) a.ctx[c.b * (long long)(a.c.heads * HD) + (long long)c.h * HD + tid] = sat_i16(rhu64(total, 15));
 }
 
-template <int HD>
+template <int HD, int WARPS>
 cudaError_t launch_whole(const AttendArgs& a, int parts, size_t share, cudaStream_t s) {
+  constexpr int MOST = WARPS == 8 ? FEW_SLOTS * 4 : (int)MAX_SHARE * 4;
   static std::atomic<unsigned long long> done{0};
-  cudaError_t e = allow_smem((const void*)attend_q4_kernel<HD>, (int)MAX_SHARE * 4, done);
+  cudaError_t e = allow_smem((const void*)attend_q4_kernel<HD, WARPS>, MOST, done);
   if (e == cudaSuccess && parts > 8)
-    e = cudaFuncSetAttribute(attend_q4_kernel<HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(attend_q4_kernel<HD, WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -705,12 +723,12 @@ cudaError_t launch_whole(const AttendArgs& a, int parts, size_t share, cudaStrea
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.c.batch * a.c.heads * (size_t)parts));
-  cfg.blockDim = dim3(WHOLE_THREADS);
+  cfg.blockDim = dim3(32 * WARPS);
   cfg.dynamicSmemBytes = share * sizeof(int32_t);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = parts > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, attend_q4_kernel<HD>, a);
+  return cudaLaunchKernelEx(&cfg, attend_q4_kernel<HD, WARPS>, a);
 }
 
 template <int HD>
@@ -730,11 +748,21 @@ struct Q4Plan {
   size_t logits, chunk_max, chunk_sum, arrived, partial, total;  // scratch offsets and size
 };
 
+// WHOLE unless rows are so few that clusters of 16 would be wanted (8 a row
+// leave SMs idle) and so long that such a CTA would have over FEW_SLOTS slots:
+// clusters of 16 fill the SMs badly.  Microseconds of WHOLE and of split, 64
+// dims, scores kept: 8 rows of 131,072 41 and 34, of 65,536 27 and 28; 16 rows
+// of 40,960 35 and 30; one row of 262,144 51 and 30; 32 rows of 16,384 22 and 28;
+// 64 rows of 16,384 29 and 34; 256 rows of 8,320 39 and 49; 2,048 rows 256 and 330.
+//
+// A CTA of WHOLE has 8 warps up to FEW_SLOTS slots, 16 above (twice as many CTAs
+// an SM, or half as many steps of a row): 512 rows of 1,024 x 16 dims take 12.8
+// us with 8 and 16.7 with 16, 512 of 2,048 x 64 25.1 and 27.1; 256 of 8,320 x 64
+// 52 and 39.
 Q4Plan plan_of(const nsrl_q4_cache& c) {
   Q4Plan p{};
-  const size_t bh = c.batch * c.heads, groups = std::max<size_t>(1, c.head_dim / 32);
-  const size_t bytes = bh * c.capacity * (c.head_dim + 8 * groups);
-  p.split = bytes >= SPLIT_BYTES;
+  const size_t bh = c.batch * c.heads;
+  p.split = bh * 8 < 148 && c.capacity >= SPLIT_SLOTS;
   p.parts = 1;
   if (!p.split) {
     while (p.parts < MAX_CLUSTER && ((c.capacity + p.parts - 1) / p.parts > MAX_SHARE ||
@@ -784,9 +812,10 @@ cudaError_t launch_attend_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache& 
     e = c.head_dim == 16 ? launch_split<16>(a, s) : c.head_dim == 64 ? launch_split<64>(a, s) : launch_split<256>(a, s);
   } else {
     const size_t share = ((c.capacity + p.parts - 1) / p.parts + UNIT - 1) / UNIT * UNIT;
-    e = c.head_dim == 16   ? launch_whole<16>(a, p.parts, share, s)
-        : c.head_dim == 64 ? launch_whole<64>(a, p.parts, share, s)
-                           : launch_whole<256>(a, p.parts, share, s);
+    const bool few = share <= FEW_SLOTS;
+    e = c.head_dim == 16   ? (few ? launch_whole<16, 8>(a, p.parts, share, s) : launch_whole<16, 16>(a, p.parts, share, s))
+        : c.head_dim == 64 ? (few ? launch_whole<64, 8>(a, p.parts, share, s) : launch_whole<64, 16>(a, p.parts, share, s))
+                           : (few ? launch_whole<256, 8>(a, p.parts, share, s) : launch_whole<256, 16>(a, p.parts, share, s));
   }
   return e != cudaSuccess ? e : cudaGetLastError();
 }

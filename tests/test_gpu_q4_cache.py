@@ -124,9 +124,12 @@ def test_read_saturates_and_refuses(K):
 ATTENDS = [(1, 1, 64, 16, [1]), (2, 3, 64, 64, [31, 33]), (3, 2, 16, 48, [1, 17, 48]), (2, 2, 256, 160, [160, 129]),
            (1, 4, 64, 1024, [1000]), (4, 16, 64, 2048, [2048, 1, 2047, 1025]), (1, 1, 16, 4096, [4095]),
            (40, 8, 64, 272, None), (160, 1, 16, 80, None), (1, 2, 256, 2064, [2050]), (2, 1, 64, 8208, [8193, 64])]
-# large enough for the split form: ragged rows of one chunk, of several, and that end with or just past one
-ATTENDS += [(80, 1, 64, 4112, None), (40, 2, 64, 4112, [1, 2048, 2049, 4096, 4097, 4112, 31, 256] * 5),
-            (130, 2, 16, 4112, None), (20, 2, 256, 2064, None)]
+# few rows and long enough for the split form: ragged rows of one chunk, of several, and that end with or just past one
+ATTENDS += [(5, 2, 64, 32784, None), (8, 1, 64, 32768, [1, 2048, 2049, 4096, 4097, 32768, 31, 256]),
+            (3, 2, 16, 36880, None), (2, 2, 256, 32784, [32783, 20481]), (1, 18, 16, 34000, [33999])]
+# one below that, and as long of more rows than it takes
+ATTENDS += [(2, 2, 64, 32752, None), (19, 1, 16, 32768, None), (10, 2, 64, 32784, None), (130, 2, 16, 4112, None),
+            (150, 1, 64, 2064, None), (75, 2, 256, 592, None)]
 
 
 @pytest.mark.parametrize("case", ATTENDS)

@@ -136,7 +136,7 @@ def test_attend_refusals(lib):
         args[i] = None
         assert f(*args) == 1
     assert f(None, 256, q4(batch=0), None, None, None, 0, None, None) == 0
-    big = q4(batch=64, capacity=8192)  # takes a workspace
+    big = q4(batch=16, capacity=32768)  # takes a workspace
     ws = lib.nsrl_attention_decode_q4_workspace_size(big)
     assert ws >= 4 * 64 * 4 * 8192
     for w, n in ((None, ws), (P16, ws), (C.c_void_p(256), ws - 1)):
