@@ -136,9 +136,9 @@ def test_attend_refusals(lib):
         args[i] = None
         assert f(*args) == 1
     assert f(None, 256, q4(batch=0), None, None, None, 0, None, None) == 0
-    big = q4(batch=16, capacity=32768)  # takes a workspace
+    big = q4(batch=4, capacity=65536)  # takes a workspace
     ws = lib.nsrl_attention_decode_q4_workspace_size(big)
-    assert ws >= 4 * 64 * 4 * 8192
+    assert ws >= 4 * 16 * 65536
     for w, n in ((None, ws), (P16, ws), (C.c_void_p(256), ws - 1)):
         assert f(P16, 256, big, P16, P16, w, n, P16, None) == 1
 
