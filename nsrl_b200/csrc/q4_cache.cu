@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(THREADS) q4_read_kernel(const ReadArgs a) {
 // q4_move_kernel copies the m-th listed slot into the m-th hole.  Sources lie
 // at or past `keep` and destinations below it, so the moves need no order.
 constexpr unsigned SAFE = 0x80000000u;  // key of a protected slot, above every score
-constexpr unsigned NONE = 0xFFFFFFFFu;  // no slot
+constexpr int SELECT_HELD = 16;         // keys of a lane in registers
+constexpr int SELECT_WARPS = 20;        // of a CTA, at most: 48 registers a thread
 
 struct EvictArgs {
   nsrl_q4_cache c;
@@ -178,22 +179,26 @@ struct EvictArgs {
   nsrl_device_status* st;
 };
 
-// The first HELD slots of a thread's span stay in registers (loaded all at once:
-// the loads' latency is most of a short row's time); a longer span's others are
-// read again in each pass.  Bound by memory: 8 bytes a slot in, 8 a kept slot out.
-template <int SEL_THREADS, int HELD>
-__global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs a) {
-  constexpr int SEL_WARPS = SEL_THREADS / 32;
-  extern __shared__ uint32_t bitmap[];  // kept slots, 32 a word
-  __shared__ int hist[256];
-  __shared__ int warp_a[SEL_WARPS], warp_b[SEL_WARPS];
+// The first HELD keys of a lane stay in registers (loaded all at once: the loads'
+// latency is most of a short row's time); a longer span's others are made again in
+// each pass, and scores and positions are read again where they are copied.
+// Bound by instructions (some 126 a round of 32 slots at three passes, ties among
+// the last) and the barriers between passes, well above its 8 bytes a slot in and
+// 8 a kept slot out: 2,048 rows of 2,112 slots take 40 us, their bytes 10.
+__global__ void __launch_bounds__(32 * SELECT_WARPS, 2) q4_select_kernel(const EvictArgs a) {
+  constexpr int HELD = SELECT_HELD, STEP = 4;  // keys are gone through STEP rounds at a time
+  extern __shared__ uint32_t bitmap[];         // kept slots, 32 a word
+  __shared__ int hist[256 + 32];  // and a place a lane for keys that are not counted
+  __shared__ int warp_a[SELECT_WARPS], warp_b[SELECT_WARPS];
   __shared__ unsigned s_prefix, s_top;
   __shared__ int s_want, s_safe;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int threads = blockDim.x, warps = threads >> 5;
   if (tid == 0) {
     s_top = 0;
     s_safe = 0;
   }
+  for (int i = tid; i < 256; i += threads) hist[i] = 0;
   griddep_wait();
   griddep_launch();
   const unsigned bh = blockIdx.x, b = bh / (unsigned)a.c.heads;
@@ -212,50 +217,57 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
   int32_t* scores_out = a.scores_out + base;
   int32_t* positions_out = a.positions_out + base;
   if (n <= keep) {
-    for (int i = tid; i < n; i += SEL_THREADS) {
+    for (int i = tid; i < n; i += threads) {
       scores_out[i] = scores[i];
       positions_out[i] = positions[i];
     }
     if (tid == 0) a.moves[bh] = 0;
     return;
   }
-  const long long border = (long long)a.next[b] - a.recent;
+  // protected: positions up to sink, and from border on
+  const int sink = (int)min(a.sinks - 1, (long long)INT_MAX);
+  const int border = (int)max((long long)a.next[b] - a.recent, (long long)INT_MIN);
   // Each warp takes one contiguous span of slots, 32 at a time, so that ranks
   // follow the slot order.
-  const int span = ((n + SEL_WARPS - 1) / SEL_WARPS + 31) / 32 * 32;
+  const int span = ((n + warps - 1) / warps + 31) / 32 * 32;
   const int lo = min(n, warp * span), hi = min(n, lo + span);
   const int rounds = (hi - lo + 31) / 32;
   auto key_of = [&](int score, int position) -> unsigned {
-    return (long long)position < a.sinks || (long long)position >= border ? SAFE : (unsigned)max(score, 0);
+    return position <= sink || position >= border ? SAFE : (unsigned)max(score, 0);
   };
-  int score[HELD], position[HELD];
+  const int32_t* my_scores = scores + lo + lane;
+  const int32_t* my_positions = positions + lo + lane;
+  const int mine = hi - lo - lane;  // this lane's slot of round r is there if 32 r < mine
+  // A round past the span, or a slot past the row's end, has the smallest key, 0:
+  // counts of larger keys do not see it.  Where equal keys count, `mine` leaves it out.
   unsigned key[HELD];
+  {
+    int score[HELD], position[HELD];
 #pragma unroll
-  for (int k = 0; k < HELD; ++k) {
-    const int i = lo + 32 * k + lane;
-    score[k] = i < hi ? scores[i] : 0;
-    position[k] = i < hi ? positions[i] : 0;
+    for (int k = 0; k < HELD; ++k) {
+      score[k] = 32 * k < mine ? my_scores[32 * k] : 0;
+      position[k] = 32 * k < mine ? my_positions[32 * k] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) key[k] = 32 * k < mine ? key_of(score[k], position[k]) : 0;
   }
-#pragma unroll
-  for (int k = 0; k < HELD; ++k) key[k] = lo + 32 * k + lane < hi ? key_of(score[k], position[k]) : NONE;
-  // f(round, key, score, position) for every round of the warp's span; lanes past it get NONE
+  // f(round, key) for every round of the warp's span, and for some past it
   auto each = [&](auto f) {
 #pragma unroll
-    for (int k = 0; k < HELD; ++k)
-      if (k < rounds) f(k, key[k], score[k], position[k]);
-    for (int k = HELD; k < rounds; ++k) {
-      const int i = lo + 32 * k + lane;
-      const int s = i < hi ? scores[i] : 0, p = i < hi ? positions[i] : 0;
-      f(k, i < hi ? key_of(s, p) : NONE, s, p);
-    }
+    for (int k = 0; k < HELD; k += STEP)
+      if (k < rounds) {
+#pragma unroll
+        for (int m = 0; m < STEP; ++m) f(k + m, key[k + m]);
+      }
+    for (int k = HELD; k < rounds; ++k) f(k, 32 * k < mine ? key_of(my_scores[32 * k], my_positions[32 * k]) : 0);
   };
 
   // ---- the protected slots, and the largest other key ----
   int safe = 0;
   unsigned top = 0;
-  each([&](int, unsigned k, int, int) {
-    safe += k == SAFE;
-    top = max(top, k < SAFE ? k : 0u);
+  each([&](int, unsigned k) {
+    safe += (int)(k >> 31);
+    top = max(top, k & ~SAFE);
   });
   safe = __reduce_add_sync(0xffffffffu, safe);
   top = __reduce_max_sync(0xffffffffu, top);
@@ -272,12 +284,10 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
     want = keep - s_safe;
     unsigned prefix = 0;
     int shift = s_top == 0 ? 0 : max(0, 24 - __clz(s_top));  // the top eight bits in use first
-    int fixed = 31;  // the bits of `prefix` from here up are settled
+    int fixed = 31;  // the bits of `prefix` from here up are settled (SAFE has bit 31, `prefix` has not)
     for (;;) {
-      for (int i = tid; i < 256; i += SEL_THREADS) hist[i] = 0;
-      __syncthreads();
-      each([&](int, unsigned k, int, int) {
-        if (k < SAFE && (k >> fixed) == (prefix >> fixed)) atomicAdd(&hist[(k >> shift) & 255], 1);
+      each([&](int, unsigned k) {
+        atomicAdd(&hist[(k ^ prefix) >> fixed ? 256 + lane : (k >> shift) & 255], 1);
       });
       __syncthreads();
       if (warp == 0) {
@@ -295,21 +305,23 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
           if (lane >= o) before += v;
         }
         before -= sum;  // keys in higher bins of other lanes
+        if (before < want && before + sum >= want) {  // one lane: its bins hold the want-th key
+          int j = 0;
+          while (before + own[0] < want) {
+            before += own[0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (before < want && before + own[j] >= want) {
-            s_prefix = (prefix & ~(255u << shift)) | (unsigned)(255 - 8 * lane - j) << shift;
-            s_want = want - before;
-            s_top = (unsigned)own[j];
+            for (int m = 0; m < 7; ++m) own[m] = own[m + 1];
+            ++j;
           }
-          before += own[j];
+          s_prefix = (prefix & ~(255u << shift)) | (unsigned)(255 - 8 * lane - j) << shift;
+          s_want = want - before;
+          s_top = (unsigned)own[0];
         }
       }
       __syncthreads();
       prefix = s_prefix;
       want = s_want;
       const bool all = want == (int)s_top;  // every key of the bin stays: what lies above prefix - 1
-      __syncthreads();
       if (all && prefix > 0) {
         last = prefix - 1;
         want = 0;
@@ -321,66 +333,99 @@ __global__ void __launch_bounds__(SEL_THREADS) q4_select_kernel(const EvictArgs 
       }
       fixed = shift;
       shift = max(0, shift - 8);
+      for (int i = tid; i < 256; i += threads) hist[i] = 0;
+      __syncthreads();
     }
   }
 
-  auto prefix_of_warps = [&](const int* mine) {  // exclusive prefix of warp counts
-    int s = 0;
-    for (int w = 0; w < warp; ++w) s += mine[w];
-    return s;
+  auto prefix_of_warps = [&](int mine) {  // exclusive prefix over the warps of lane w's count of warp w
+    int before = lane < warp ? mine : 0;
+    return __reduce_add_sync(0xffffffffu, before);
   };
-  int rank = 0;
-  if (want > 0) {  // ties go to the lower slots
+  const unsigned under = (1u << lane) - 1;
+  int cutoff = lo;   // of the slots whose key is `last`, those below it stay: ties go to the lower slots
+  if (want > 0) {
     int equal = 0;
-    each([&](int, unsigned k, int, int) { equal += k == last; });
+    each([&](int r, unsigned k) { equal += k == last && 32 * r < mine; });
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) warp_a[warp] = equal;
     __syncthreads();
-    rank = prefix_of_warps(warp_a);
+    int rank = prefix_of_warps(lane < warps ? warp_a[lane] : 0);
     __syncthreads();
-  }
-  const unsigned under = (1u << lane) - 1;
-  int holes = 0, late = 0;
-  each([&](int r, unsigned k, int s, int p) {
-    const int i = lo + 32 * r + lane;
-    bool kept = k != NONE && k > last;
-    if (want > 0) {
-      const unsigned eq = __ballot_sync(0xffffffffu, k == last);
-      kept = kept || (k == last && rank + __popc(eq & under) < want);
-      rank += __popc(eq);
+    if (rank + equal <= want)
+      cutoff = hi;
+    else if (rank < want) {  // this warp has the last of them
+      each([&](int r, unsigned k) {
+        const bool tie = k == last && 32 * r < mine;
+        const unsigned eq = __ballot_sync(0xffffffffu, tie);
+        if (tie && rank + __popc(eq & under) < want) cutoff = lo + 32 * r + lane + 1;
+        rank += __popc(eq);
+      });
+      cutoff = __reduce_max_sync(0xffffffffu, cutoff);
     }
+  }
+  const bool copy_scores = scores_out != scores, copy_positions = positions_out != positions;
+  int32_t* my_scores_out = scores_out + lo + lane;
+  int32_t* my_positions_out = positions_out + lo + lane;
+  const int ties = cutoff - lo - lane, low = min(keep, hi) - lo - lane;
+  each([&](int r, unsigned k) {
+    const bool kept = k > last || (k == last && 32 * r < ties);
     const unsigned bits = __ballot_sync(0xffffffffu, kept);
-    if (lane == 0) bitmap[(lo >> 5) + r] = bits;
-    // of the round's slots, those below `keep`
-    const int low = max(0, min(32, keep - (lo + 32 * r))), live = min(32, hi - (lo + 32 * r));
-    const unsigned low_mask = low >= 32 ? 0xffffffffu : (1u << low) - 1;
-    const unsigned live_mask = live >= 32 ? 0xffffffffu : (1u << live) - 1;
-    holes += __popc(~bits & low_mask & live_mask);
-    late += __popc(bits & ~low_mask);
-    if (kept && i < keep) {
-      if (scores_out != scores) scores_out[i] = s;
-      if (positions_out != positions) positions_out[i] = p;
+    if (lane == 0 && r < rounds) bitmap[(lo >> 5) + r] = bits;
+    if (kept && 32 * r < low) {
+      if (copy_scores) my_scores_out[32 * r] = my_scores[32 * r];
+      if (copy_positions) my_positions_out[32 * r] = my_positions[32 * r];
     }
   });
+  __syncwarp();
+  // A lane takes a word of the warp's part of the bitmap: its holes below `keep`, and its kept slots at or past it.
+  auto word = [&](int r, unsigned& hole, unsigned& late) {
+    const int first = lo + 32 * r;
+    const unsigned bits = r < rounds ? bitmap[first >> 5] : 0;
+    const int low = max(0, min(32, keep - first)), live = max(0, min(32, hi - first));
+    const unsigned low_mask = low >= 32 ? 0xffffffffu : (1u << low) - 1;
+    const unsigned live_mask = live >= 32 ? 0xffffffffu : (1u << live) - 1;
+    hole = ~bits & low_mask & live_mask;
+    late = bits & ~low_mask;
+  };
+  int holes = 0, lates = 0;
+  for (int r = lane; r < rounds; r += 32) {
+    unsigned hole, late;
+    word(r, hole, late);
+    holes += __popc(hole);
+    lates += __popc(late);
+  }
+  holes = __reduce_add_sync(0xffffffffu, holes);
+  lates = __reduce_add_sync(0xffffffffu, lates);
   if (lane == 0) {
     warp_a[warp] = holes;
-    warp_b[warp] = late;
+    warp_b[warp] = lates;
   }
   __syncthreads();
-  int hole_rank = prefix_of_warps(warp_a), late_rank = prefix_of_warps(warp_b);
+  int hole_rank = prefix_of_warps(lane < warps ? warp_a[lane] : 0);
+  int late_rank = prefix_of_warps(lane < warps ? warp_b[lane] : 0);
   int2* list = a.list + (size_t)bh * a.most;
-  for (int r = 0; r < rounds; ++r) {
-    const int i = lo + 32 * r + lane;
-    const unsigned bits = bitmap[(lo >> 5) + r];
-    const bool kept = (bits >> lane) & 1;
-    const bool hole = i < hi && i < keep && !kept, moves = i < hi && i >= keep && kept;
-    const unsigned hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, moves);
-    if (hole) list[hole_rank + __popc(hb & under)].y = i;
-    if (moves) list[late_rank + __popc(mb & under)].x = i;
-    hole_rank += __popc(hb);
-    late_rank += __popc(mb);
+  for (int r0 = 0; r0 < rounds; r0 += 32) {
+    unsigned hole, late;
+    word(r0 + lane, hole, late);
+    // both counts in one scan: at most 1,024 each
+    const unsigned both = (unsigned)__popc(hole) | (unsigned)__popc(late) << 16;
+    unsigned upto = both;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned total = __shfl_sync(0xffffffffu, upto, 31);
+    const int first = lo + 32 * (r0 + lane);
+    int at = hole_rank + (int)((upto - both) & 0xFFFF);
+    for (; hole; hole &= hole - 1) list[at++].y = first + __ffs((int)hole) - 1;
+    at = late_rank + (int)((upto - both) >> 16);
+    for (; late; late &= late - 1) list[at++].x = first + __ffs((int)late) - 1;
+    hole_rank += (int)(total & 0xFFFF);
+    late_rank += (int)(total >> 16);
   }
-  if (tid == SEL_THREADS - 1) a.moves[bh] = late_rank;  // the last warp's running rank is the total
+  if (tid == threads - 1) a.moves[bh] = late_rank;  // the last warp's running rank is the total
 }
 
 // A move is 2 head_dim / 2 code bytes, the scales, the score and the position:
@@ -520,17 +565,11 @@ cudaError_t launch_q4_evict(const nsrl_q4_cache& c, const int32_t* lens, const i
   a.st = st;
   const size_t smem = (c.capacity / 32 + 1) * sizeof(uint32_t);
   {
-    // Threads follow the capacity, 16 slots a thread up to 16,384: several CTAs an
-    // SM hide each other's barriers (2,048 rows of 2,112 slots took 96 us in 1,024
-    // threads that read their keys again each pass).
-    const unsigned threads = c.capacity <= 2048 ? 128 : c.capacity <= 4096 ? 256 : c.capacity <= 8192 ? 512 : 1024;
-    auto* kernel = threads == 128   ? q4_select_kernel<128, 16>
-                   : threads == 256 ? q4_select_kernel<256, 16>
-                   : threads == 512 ? q4_select_kernel<512, 16>
-                                    : q4_select_kernel<1024, 16>;
+    // Warps follow the capacity, one for the keys that its lanes hold, four at least.
+    const size_t warps = std::min<size_t>(SELECT_WARPS, std::max<size_t>(4, (c.capacity + 32 * SELECT_HELD - 1) / (32 * SELECT_HELD)));
     ProfScope prof("q4_select", s, 0.0, 8.0 * (double)bh * (double)c.capacity);
     // the bitmap of the largest capacity is 32 KB: within the default limit
-    const cudaError_t e = launch_pdl(kernel, dim3((unsigned)bh), dim3(threads), smem, s, a);
+    const cudaError_t e = launch_pdl(q4_select_kernel, dim3((unsigned)bh), dim3(32 * (unsigned)warps), smem, s, a);
     if (e != cudaSuccess) return e;
   }
   // moves of a CTA's step: 128 (32 at 256 dims), as many CTAs a row as its moves may need, 64 at most
