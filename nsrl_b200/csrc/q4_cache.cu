@@ -118,6 +118,11 @@ struct ReadArgs {
   nsrl_device_status* st;
 };
 
+// Rows of a thread, loaded before the first is written: 2,048 rows of 2,048 slots
+// take 245 us one at a time and 218 two or four at a time (99% of copy
+// bandwidth); 2,048 single slots 5.5, 5.5 and 7.
+constexpr int READ_ROWS = 2;
+
 __device__ __forceinline__ uint4 dequantise8(uint32_t codes, uint32_t scale_word) {
   const int scale = (int)(scale_word & 0xFFFF), zero = (int)(int16_t)(scale_word >> 16);
   uint32_t w[4];
@@ -132,25 +137,39 @@ __global__ void __launch_bounds__(THREADS) q4_read_kernel(const ReadArgs a) {
   constexpr int LPR = HD / 8;
   constexpr int LPG = HD < 32 ? HD / 8 : 4;
   constexpr int G = HD < 32 ? 1 : HD / 32;
+  constexpr int U = READ_ROWS, PER = THREADS / LPR;
   griddep_wait();
   griddep_launch();
   const int sub = threadIdx.x % LPR;
-  const unsigned row = blockIdx.x * (THREADS / LPR) + threadIdx.x / LPR;
-  if (row >= a.rows) return;
   const unsigned tokens = (unsigned)a.tokens;
-  const unsigned bh = row / tokens, t = row - bh * tokens, b = bh / (unsigned)a.c.heads;
-  const size_t i = (size_t)row * LPR + sub;
-  const long long start = a.starts ? (long long)a.starts[b] : 0;
-  if (start < 0 || start + a.tokens > (long long)a.c.capacity) {
-    if (t == 0 && sub == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
-    return;
+  uint32_t ck[U], cv[U], sk[U], sv[U];
+  bool ok[U];
+  const unsigned row0 = blockIdx.x * (PER * U) + threadIdx.x / LPR;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned row = row0 + u * PER;
+    ok[u] = row < a.rows;
+    if (!ok[u]) continue;
+    const unsigned bh = row / tokens, t = row - bh * tokens, b = bh / (unsigned)a.c.heads;
+    const long long start = a.starts ? (long long)a.starts[b] : 0;
+    if (start < 0 || start + a.tokens > (long long)a.c.capacity) {
+      if (t == 0 && sub == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
+      ok[u] = false;
+      continue;
+    }
+    const size_t slot = (size_t)bh * a.c.capacity + (size_t)(start + t);
+    ck[u] = reinterpret_cast<const uint32_t*>(a.c.k_codes)[slot * LPR + sub];
+    cv[u] = reinterpret_cast<const uint32_t*>(a.c.v_codes)[slot * LPR + sub];
+    sk[u] = a.c.k_scales[slot * G + sub / LPG];
+    sv[u] = a.c.v_scales[slot * G + sub / LPG];
   }
-  const size_t slot = (size_t)bh * a.c.capacity + (size_t)(start + t);
-  const uint32_t ck = reinterpret_cast<const uint32_t*>(a.c.k_codes)[slot * LPR + sub];
-  const uint32_t cv = reinterpret_cast<const uint32_t*>(a.c.v_codes)[slot * LPR + sub];
-  const uint32_t sk = a.c.k_scales[slot * G + sub / LPG], sv = a.c.v_scales[slot * G + sub / LPG];
-  reinterpret_cast<uint4*>(a.k)[i] = dequantise8(ck, sk);
-  reinterpret_cast<uint4*>(a.v)[i] = dequantise8(cv, sv);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (!ok[u]) continue;
+    const size_t i = (size_t)(row0 + u * PER) * LPR + sub;
+    reinterpret_cast<uint4*>(a.k)[i] = dequantise8(ck[u], sk[u]);
+    reinterpret_cast<uint4*>(a.v)[i] = dequantise8(cv[u], sv[u]);
+  }
 }
 
 // ------------------------------------------------------------- eviction ----
@@ -529,7 +548,7 @@ cudaError_t launch_q4_append(const nsrl_q4_cache& c, const int16_t* k, const int
 
 cudaError_t launch_q4_read(const nsrl_q4_cache& c, const int32_t* starts, size_t tokens, int16_t* k, int16_t* v,
                            nsrl_device_status* st, cudaStream_t s) {
-  const size_t n = c.batch * c.heads * tokens, per_block = THREADS / (c.head_dim / 8);
+  const size_t n = c.batch * c.heads * tokens, per_block = READ_ROWS * THREADS / (c.head_dim / 8);
   if (n == 0) return cudaSuccess;
   if (n > 0xffffff00u) return cudaErrorInvalidValue;  // the entry point refuses it
   const ReadArgs a{c, starts, (long long)tokens, (unsigned)n, k, v, st};
