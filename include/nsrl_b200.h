@@ -283,13 +283,15 @@ nsrl_status nsrl_q4_cache_read(const nsrl_q4_cache* cache, const int32_t* starts
 /* nsrl_attention_decode over the 4-bit cache: sequence b's query (row b of q,
  * stride ldq elements, head h at column h * head_dim) attends over the first
  * lens[b] slots (device int32, in 1..capacity), with their dequantised values
- * in place of int16 ones; the same logits, base-2 softmax and rounding, so on
- * equal values the same context.  ctx: [batch][heads * head_dim].  With
+ * (zero + scale * code; hand-made scales do not saturate here) in place of
+ * int16 ones; the same logits, base-2 softmax and rounding, so on equal values
+ * the same context.  ctx: [batch][heads * head_dim].  With
  * cache->scores, the Q15 weight of each slot is added to its score
  * (saturating at 2^31 - 1).  Capacity at most nsrl_q4_cache_max_capacity().
  * workspace: nsrl_attention_decode_q4_workspace_size(cache) bytes (0 for a
  * small cache: NULL is fine then), 256-byte aligned, its contents of no
- * account before and after. */
+ * account before and after; calls that may run at the same time, two captured
+ * graphs among them, each take one of their own. */
 size_t nsrl_q4_cache_max_capacity(void);
 size_t nsrl_attention_decode_q4_workspace_size(const nsrl_q4_cache* cache);
 nsrl_status nsrl_attention_decode_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache* cache, const int32_t* lens,

@@ -9,6 +9,10 @@ A slot of 64 dims takes 80 bytes (key and value) where the int16 cache takes
 without waiting (they may be captured into a graph; the device status tells
 rejections later).  The methods without the prefix wait and return None when
 the call was rejected, as the functions of `core` do.
+
+Calls on one cache run one after another: on one stream, or on several that the
+caller orders.  Attention without scores only reads the cache, so it may run on
+several streams at once, each call with a workspace of its own.
 """
 from __future__ import annotations
 
@@ -110,8 +114,9 @@ class Q4Cache:
         return core._raw_stream(self._dev)
 
     # ---- enqueue only
-    def launch_append(self, k, v, starts, counts=None, positions=None, status: core.Status = None) -> int:
-        """k, v: int16 [batch * tokens, heads * head_dim] of one row stride (nsrl_q4_cache_append)."""
+    def launch_append(self, k, v, starts, counts, positions, status: core.Status) -> int:
+        """k, v: int16 [batch * tokens, heads * head_dim] of one row stride; counts
+        and positions may be None (nsrl_q4_cache_append)."""
         rows, cols = k.shape[0], self._cols
         if rows % max(1, self.batch) or k.shape[1] != cols or v.shape[1] != cols:
             raise core.NsrlError("k and v must be [batch * tokens, heads * head_dim]")
@@ -137,15 +142,23 @@ class Q4Cache:
                                          core._array(v, torch.int16, shape, self._dev, "v"), status.buf.data_ptr(),
                                          stream)
 
-    def launch_attend(self, q, lens, ctx, status: core.Status) -> int:
-        """q: int16 [batch, heads * head_dim] rows, ctx likewise and contiguous (nsrl_attention_decode_q4)."""
+    def attend_workspace_bytes(self) -> int:
+        return self._ws_bytes
+
+    def launch_attend(self, q, lens, ctx, status: core.Status, ws=None) -> int:
+        """q: int16 [batch, heads * head_dim] rows, ctx likewise and contiguous; ws:
+        attend_workspace_bytes() of uint8, the cache's own by default
+        (nsrl_attention_decode_q4)."""
         stream, cols = self._stream(), self._cols
+        wp, wn = self._ws_ptr, self._ws_bytes
+        if ws is not None:
+            wp, wn = core._array(ws, torch.uint8, ws.shape, self._dev, "the workspace"), ws.numel()
         qp = core._rows(q, self.batch, cols, self._dev, "q")
         if q.shape[1] != cols:
             raise core.NsrlError("q must be [batch, heads * head_dim]")
         return _lib().nsrl_attention_decode_q4(qp, core._row_stride(q), self._ref, self._per_sequence(lens, "lens"),
                                                core._array(ctx, torch.int16, (self.batch, cols), self._dev, "ctx"),
-                                               self._ws_ptr, self._ws_bytes, status.buf.data_ptr(), stream)
+                                               wp, wn, status.buf.data_ptr(), stream)
 
     def evict_workspace_bytes(self, keep: int) -> int:
         return _lib().nsrl_q4_cache_evict_workspace_size(self._ref, keep)
@@ -206,6 +219,11 @@ def prenorm_attention_decode_block_q4(x, rms_gamma, rms_eps, q, k, v, o, cache: 
     B, d = x.shape
     if B != cache.batch or g.numel() != d:
         raise core.NsrlError("x must be [cache.batch, d] and rms_gamma [d]")
+    if rotary is not None:
+        if rotary.head_dim != cache.head_dim:
+            raise core.NsrlError(f"the rotary plan is for head_dim {rotary.head_dim}, the cache has {cache.head_dim}")
+        if rotary.turns.get_device() != cache._dev:
+            raise core.NsrlError(f"the rotary plan is on {rotary.turns.device}, the cache on {cache.device}")
     stream = cache._stream()
     xp = core._rows(x, B, d, cache._dev, "x")
     lp = cache._per_sequence(lens, "lens")

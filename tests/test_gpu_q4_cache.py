@@ -185,7 +185,7 @@ def test_attend_long_stream(K):
     cap = 100000
     cache, kv, vv = filled(K, rng, 1, 1, 64, cap, True, 8, 4096)
     q = gaussian(rng, (1, 1, 64), 8)
-    for n in (cap, 50001):  # eight CTAs of a cluster
+    for n in (cap, 50001):
         ctx, scores = P.attend(q, kv, vv, [n], host(cache.scores))
         assert np.array_equal(host(cache.attend(dev(q.reshape(1, 64)), i32([n]))), ctx)
         assert np.array_equal(host(cache.scores), scores)
@@ -201,6 +201,60 @@ def test_attend_long_streams_split(K):
         ctx, scores = P.attend(q, kv, vv, [n], host(cache.scores))
         assert np.array_equal(host(cache.attend(dev(q.reshape(1, 256)), i32([n]))), ctx)
         assert np.array_equal(host(cache.scores), scores)
+
+
+@pytest.mark.parametrize("B,cap", [(150, 32768), (19, 262144)])  # one CTA a row, and eight
+def test_attend_largest_shares(K, B, cap):
+    """32,768 slots a CTA: the most logits that one keeps."""
+    g = torch.Generator(device="cuda").manual_seed(cap)
+    draw = lambda lo, hi, shape, t: torch.randint(lo, hi, shape, generator=g, device="cuda").to(t)  # noqa: E731
+    kc, vc = (draw(0, 256, (B, 1, cap, 8), torch.uint8) for _ in "kv")
+    ks = draw(1, 9, (B, 1, cap, 1), torch.int32) | (draw(-60, 1, (B, 1, cap, 1), torch.int32) << 16)
+    vs = draw(1, 1000, (B, 1, cap, 1), torch.int32) | (draw(-9000, 1, (B, 1, cap, 1), torch.int32) << 16)
+    old = draw(0, 1 << 20, (B, 1, cap), torch.int32)
+    cache = K.Q4Cache.of(kc, vc, ks, vs, old.clone())
+    q = draw(-40, 41, (B, 16), torch.int16)
+    lens = [cap - 7 * b for b in range(B)]
+    ctx = cache.attend(q, i32(lens))
+    k, v = cache.read(cap)
+    for b in (0, 1, B - 1):
+        one = slice(b, b + 1)
+        want, scores = P.attend(host(q[one]).reshape(1, 1, 16), host(k[one]), host(v[one]), lens[one], host(old[one]))
+        assert np.array_equal(host(ctx[one]), want)
+        assert np.array_equal(host(cache.scores[one]), scores)
+
+
+def test_attend_graphs_side_by_side(K):
+    """Two captured calls on a cache without scores, each with its own workspace, replayed at once."""
+    from nsrl_b200 import core
+    rng = np.random.default_rng(17)
+    B, H, cap = 1, 2, 40000
+    cache, _, _ = filled(K, rng, B, H, 64, cap, False, 8, 4096)
+    q = [dev(gaussian(rng, (B, H * 64), 8)) for _ in range(2)]
+    lens = [i32([cap]), i32([33333])]
+    want = [host(cache.attend(q[i], lens[i])) for i in range(2)]
+    ctx = [torch.zeros((B, H * 64), dtype=torch.int16, device="cuda") for _ in range(2)]
+    assert cache.attend_workspace_bytes() > 0
+    ws = [torch.empty(cache.attend_workspace_bytes(), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    st = [core.Status() for _ in range(2)]
+    streams, graphs = [torch.cuda.Stream() for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], stream=streams[i]):
+            assert cache.launch_attend(q[i], lens[i], ctx[i], st[i], ws[i]) == 0
+    for _ in range(8):
+        for c in ctx:
+            c.zero_()
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert np.array_equal(host(ctx[i]), want[i])
+    with pytest.raises(core.NsrlError):
+        cache.launch_attend(q[0], lens[0], ctx[0], st[0], ws[0].view(torch.int32))
+    assert cache.launch_attend(q[0], lens[0], ctx[0], st[0], ws[0][:256]) != 0
 
 
 def test_scores_saturate(K):
@@ -454,3 +508,15 @@ def test_decode_block_rejects_a_full_cache(K):
     gamma = torch.full((128,), 30000, dtype=torch.int16, device="cuda")
     assert K.prenorm_attention_decode_block_q4(x, gamma, 1, lin, lin, lin, lin, cache, i32([15])) is not None
     assert K.prenorm_attention_decode_block_q4(x, gamma, 1, lin, lin, lin, lin, cache, i32([16])) is None
+
+
+def test_decode_block_refuses_another_plan(K):
+    from nsrl_b200 import core, rotary, synth as Y
+    cache = K.Q4Cache(1, 2, 64, 16)
+    lin = core.Linear(torch.from_numpy(Y.i8_uniform(1, (128, 128))), core.make_scales(1, 12, 128))
+    x = dev(Y.q15_gaussian(3, (1, 128)))
+    gamma = torch.full((128,), 30000, dtype=torch.int16, device="cuda")
+    args = (x, gamma, 1, lin, lin, lin, lin, cache, i32([0]), None)
+    with pytest.raises(core.NsrlError):
+        K.prenorm_attention_decode_block_q4(*args, rotary.Rotary(16))
+    assert K.prenorm_attention_decode_block_q4(*args, rotary.Rotary(64)) is not None
