@@ -12,6 +12,7 @@
 //           where rows are few: each takes a contiguous share of the slots,
 //           keeps their logits in shared memory, and the cluster exchanges
 //           maximum, sum and partial contexts through distributed shared memory.
+//           Many rows of unlike lengths begin with the longest (order_kernel).
 //   split   three launches over fixed chunks of slots: KEYS writes logits (4
 //           bytes a slot) and each chunk's maximum, sums_kernel each chunk's
 //           sum, VALUES each chunk's context; the last chunk of a row to arrive
@@ -48,6 +49,9 @@ namespace {
 
 constexpr int MAX_CLUSTER = 16;
 constexpr int UNIT = 32;             // slots of a warp's step
+constexpr int LENGTHS = 64;          // classes of length
+constexpr size_t SORT_ROWS = 592, SORT_BATCH = 4096;  // from so many rows, up to so many sequences: long ones first
+constexpr size_t MANY_ROWS = 888, MANY_SLOTS = 10240;  // from so many rows up to so many slots: 8 warps a CTA
 constexpr size_t MAX_SHARE = 32768;  // logits of a CTA: 128 KB
 constexpr int CHUNK = 2048;          // slots of a CTA of the split form
 constexpr int FEW_SLOTS = 2048;      // up to which a CTA of the one-launch form has 8 warps, 16 above
@@ -70,6 +74,9 @@ struct AttendArgs {
   int len_offset;
   int16_t* ctx;
   nsrl_device_status* st;
+  // WHOLE's scratch
+  int2* order;       // [batch]: (sequence, length), the longest first; NULL: as they come
+  int length_shift;  // class of a length
   // the split form's scratch
   int chunks;           // of a row of `capacity` slots
   int32_t* logits;      // [batch * heads][capacity]
@@ -498,6 +505,32 @@ __device__ __forceinline__ void share_out(const cg::cluster_group& cluster, T* v
   cluster.sync();
 }
 
+// The sequences by class of length, the longest first, so that the call does not
+// end on a long one that began late.  Within a class in any order: a row's
+// results do not depend on when it runs.
+__global__ void __launch_bounds__(1024) q4_order_kernel(const AttendArgs a) {
+  __shared__ int count[LENGTHS], next[LENGTHS];
+  const int tid = threadIdx.x, batch = (int)a.c.batch;
+  if (tid < LENGTHS) count[tid] = 0;
+  griddep_wait();
+  griddep_launch();
+  __syncthreads();
+  auto length = [&](int i) { return (int)min((long long)a.lens[i] + a.len_offset, (long long)INT_MAX); };
+  auto length_class = [&](int len) { return min(max(len, 0) >> a.length_shift, LENGTHS - 1); };
+  for (int i = tid; i < batch; i += 1024) atomicAdd(&count[length_class(length(i))], 1);
+  __syncthreads();
+  if (tid < LENGTHS) {
+    int longer = 0;
+    for (int k = tid + 1; k < LENGTHS; ++k) longer += count[k];
+    next[tid] = longer;
+  }
+  __syncthreads();
+  for (int i = tid; i < batch; i += 1024) {
+    const int len = length(i);
+    a.order[atomicAdd(&next[length_class(len)], 1)] = make_int2(i, len);
+  }
+}
+
 template <int HD, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARPS) attend_q4_kernel(const AttendArgs a) {
   using S = Q4Shape<HD>;
@@ -518,8 +551,17 @@ __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARP
   if (tid < 128) recip[tid] = d_recip_lut[tid];
   griddep_wait();
   griddep_launch();
-  const unsigned bh = blockIdx.x / (unsigned)parts, b = bh / (unsigned)a.c.heads, h = bh - b * (unsigned)a.c.heads;
-  const long long len = (long long)a.lens[b] + a.len_offset;
+  unsigned bh = blockIdx.x / (unsigned)parts, b = bh / (unsigned)a.c.heads;
+  const unsigned h = bh - b * (unsigned)a.c.heads;
+  long long len;
+  if (a.order) {
+    const int2 o = a.order[b];
+    b = (unsigned)o.x;
+    bh = b * (unsigned)a.c.heads + h;
+    len = o.y;
+  } else {
+    len = (long long)a.lens[b] + a.len_offset;
+  }
   if (warp == 0) lay_out<HD>(query, a.q + b * a.ldq + (long long)h * HD);
   if (len <= 0 || len > (long long)a.c.capacity) {  // the same for the whole cluster
     if (tid == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
@@ -709,7 +751,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_values_ke
 
 template <int HD, int WARPS>
 cudaError_t launch_whole(const AttendArgs& a, int parts, size_t share, cudaStream_t s) {
-  constexpr int MOST = WARPS == 8 ? FEW_SLOTS * 4 : (int)MAX_SHARE * 4;
+  constexpr int MOST = 4 * (int)(WARPS == 8 ? MANY_SLOTS : MAX_SHARE);
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_smem((const void*)attend_q4_kernel<HD, WARPS>, MOST, done);
   if (e == cudaSuccess && parts > 8)
@@ -742,9 +784,10 @@ cudaError_t launch_split(const AttendArgs& a, cudaStream_t s) {
 
 // The form of a call, from what its launch knows (lengths live on the device).
 struct Q4Plan {
-  bool split;
-  int parts;      // WHOLE: CTAs of a row
-  size_t chunks;  // split: of a row
+  bool split, sorted, few;  // few: 8 warps a CTA
+  size_t share;             // slots of a CTA of WHOLE, at most
+  int parts;                // CTAs of a row
+  size_t chunks;            // split: of a row
   size_t logits, chunk_max, chunk_sum, arrived, partial, total;  // scratch offsets and size
 };
 
@@ -755,10 +798,18 @@ struct Q4Plan {
 // of 40,960 35 and 30; one row of 262,144 51 and 30; 32 rows of 16,384 22 and 28;
 // 64 rows of 16,384 29 and 34; 256 rows of 8,320 39 and 49; 2,048 rows 256 and 330.
 //
-// A CTA of WHOLE has 8 warps up to FEW_SLOTS slots, 16 above (twice as many CTAs
-// an SM, or half as many steps of a row): 512 rows of 1,024 x 16 dims take 12.8
-// us with 8 and 16.7 with 16, 512 of 2,048 x 64 25.1 and 27.1; 256 of 8,320 x 64
-// 52 and 39.
+// A CTA of WHOLE has 8 warps up to FEW_SLOTS slots, and up to MANY_SLOTS where
+// rows fill such CTAs one and a half times, 16 otherwise (half as many CTAs an
+// SM, half as many steps of a row).  8 and 16: 512 rows of 1,024 x 16 dims 12.8
+// and 16.7 us, 512 of 2,048 x 64 25.1 and 27.1; 256 of 8,320 x 64 52 and 39;
+// ragged, sorted, 640 of 8,192 56 and 51, 1,024 of 8,192 66 and 72, 2,048 of
+// 4,096 70 and 82; equal lengths, 2,048 of 4,096 121 and 130, of 8,320 234 and 231.
+//
+// From SORT_ROWS rows (two waves of 16 warps) a launch of one CTA sorts the
+// sequences by length before.  Sorted and not, ragged: 640 rows of 8,192 51 and 58
+// us, 1,280 80 and 97, 2,048 of 8,320 127 and 144; equal lengths: 90.6 and
+// 88.5, 234 and 232; 8,192 rows of 128 slots 66.9 and 64.0.  Past SORT_BATCH
+// sequences waves are so many that their end counts for little.
 Q4Plan plan_of(const nsrl_q4_cache& c) {
   Q4Plan p{};
   const size_t bh = c.batch * c.heads;
@@ -768,6 +819,10 @@ Q4Plan plan_of(const nsrl_q4_cache& c) {
     while (p.parts < MAX_CLUSTER && ((c.capacity + p.parts - 1) / p.parts > MAX_SHARE ||
                                      (bh * p.parts < 148 && c.capacity / p.parts >= 512)))
       p.parts *= 2;
+    p.share = ((c.capacity + p.parts - 1) / p.parts + UNIT - 1) / UNIT * UNIT;
+    p.few = p.share <= FEW_SLOTS || (bh >= MANY_ROWS && p.share <= MANY_SLOTS);
+    p.sorted = bh >= SORT_ROWS && c.batch > 1 && c.batch <= SORT_BATCH;
+    if (p.sorted) p.total = c.batch * sizeof(int2);
     return p;
   }
   p.chunks = (c.capacity + CHUNK - 1) / CHUNK;
@@ -795,7 +850,14 @@ cudaError_t launch_attend_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache& 
   const size_t bh = c.batch * c.heads;
   if (bh == 0) return cudaSuccess;
   if (c.capacity > q4_max_capacity() || bh > 0x7fffffffull / MAX_CLUSTER) return cudaErrorInvalidValue;
-  AttendArgs a{c, q, (long long)ldq, lens, len_offset, ctx, st};
+  AttendArgs a{};
+  a.c = c;
+  a.q = q;
+  a.ldq = (long long)ldq;
+  a.lens = lens;
+  a.len_offset = len_offset;
+  a.ctx = ctx;
+  a.st = st;
   const Q4Plan p = plan_of(c);
   const double slots = (double)bh * (double)c.capacity;
   ProfScope prof("attention_decode_q4", s, 4.0 * slots * (double)c.head_dim,
@@ -811,8 +873,14 @@ cudaError_t launch_attend_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache& 
     a.partial = reinterpret_cast<long long*>(base + p.partial);
     e = c.head_dim == 16 ? launch_split<16>(a, s) : c.head_dim == 64 ? launch_split<64>(a, s) : launch_split<256>(a, s);
   } else {
-    const size_t share = ((c.capacity + p.parts - 1) / p.parts + UNIT - 1) / UNIT * UNIT;
-    const bool few = share <= FEW_SLOTS;
+    const size_t share = p.share;
+    const bool few = p.few;
+    if (p.sorted) {
+      a.order = static_cast<int2*>(ws);
+      while (c.capacity >> a.length_shift >= LENGTHS) ++a.length_shift;
+      e = launch_pdl(q4_order_kernel, dim3(1), dim3(1024), 0, s, a);
+      if (e != cudaSuccess) return e;
+    }
     e = c.head_dim == 16   ? (few ? launch_whole<16, 8>(a, p.parts, share, s) : launch_whole<16, 16>(a, p.parts, share, s))
         : c.head_dim == 64 ? (few ? launch_whole<64, 8>(a, p.parts, share, s) : launch_whole<64, 16>(a, p.parts, share, s))
                            : (few ? launch_whole<256, 8>(a, p.parts, share, s) : launch_whole<256, 16>(a, p.parts, share, s));

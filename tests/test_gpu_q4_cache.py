@@ -130,6 +130,9 @@ ATTENDS += [(5, 2, 64, 32784, None), (8, 1, 64, 32768, [1, 2048, 2049, 4096, 409
 # one below that, and as long of more rows than it takes
 ATTENDS += [(2, 2, 64, 32752, None), (19, 1, 16, 32768, None), (10, 2, 64, 32784, None), (130, 2, 16, 4112, None),
             (150, 1, 64, 2064, None), (75, 2, 256, 592, None)]
+# rows enough to be sorted by length, and more sequences than are
+ATTENDS += [(75, 8, 16, 272, None), (300, 4, 64, 48, None), (120, 8, 16, 2064, None), (150, 4, 256, 32, None),
+            (2, 300, 64, 80, [3, 80]), (4100, 1, 16, 16, None)]
 
 
 @pytest.mark.parametrize("case", ATTENDS)
@@ -274,6 +277,16 @@ def test_attend_rejects_bad_lengths(K, lens, cap):
     q = torch.ones((2, 128), dtype=torch.int16, device="cuda")
     assert cache.attend(q, i32([5, cap])) is not None
     assert cache.attend(q, i32([cap + 1 if n < 0 and n != -3 else n for n in lens])) is None
+
+
+def test_attend_rejects_bad_lengths_among_many(K):
+    cache = K.Q4Cache(150, 4, 64, 32)
+    q = torch.ones((150, 256), dtype=torch.int16, device="cuda")
+    good = [1 + i % 32 for i in range(150)]
+    assert cache.attend_workspace_bytes() > 0 and cache.attend(q, i32(good)) is not None
+    for bad in (0, -1, 33, 2 ** 31 - 1, -2 ** 31):
+        assert cache.attend(q, i32(good[:77] + [bad] + good[78:])) is None
+    assert cache.attend(q, i32(good)) is not None
 
 
 @pytest.mark.parametrize("hd,cap", [(64, 16), (256, 16), (64, 262144), (256, 262144)])
