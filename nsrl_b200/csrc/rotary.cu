@@ -19,6 +19,11 @@
 //    the 64-bit form;
 //  - a thread keeps its column (head and pairs) and steps down the rows.
 // The loads of a thread's first rows are under way while it works out angles.
+//
+// 65,536 rows of 8 x 64 take 32 us, 4.2 TB/s: 64% of copy bandwidth, half of the
+// instructions for the angles.  A table of all 1,024 points (one load in place of
+// two, from 64 cache lines in place of 8) took 32.4, two or four angles of a thread
+// at once 32.4, 8 rows a thread no less, 48 registers 36.
 #include <algorithm>
 
 #include "common.cuh"
