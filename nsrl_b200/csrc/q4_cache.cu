@@ -11,13 +11,13 @@ namespace {
 constexpr int THREADS = 256;
 
 // ---------------------------------------------------------- append, read ---
-// A thread owns 8 dims of one (sequence, head, token), of the key and of the
-// value: a 16-byte int16 access and a 4-byte code access each.  Threads run
-// over dims, then tokens, then heads, so a warp's cache rows are contiguous
-// and its int16 rows are whole 32-byte sectors (64 dims: 128 bytes a row).
+// Append: a thread owns 16 dims of one (sequence, head, token), of the key and of
+// the value: a 32-byte sector of int16 and 8 bytes of codes each.  Threads run
+// over dims, then tokens, then heads, so a warp's cache rows are contiguous.
 // Memory has 4 hd bytes of int16 and hd + 8 ceil(hd / 32) of cache to move per
-// slot; append is bound by its 7 instructions an element (8 prompts of up to
-// 2,048 tokens, 8 x 64 dims: 13 us, and 12 to read them back).
+// slot; append is bound by its instructions, half of them for the row and its
+// scales: 8 prompts of up to 2,048 tokens, 8 x 64 dims, take 10.8 us, and 13.4
+// with 8 dims a thread.
 struct AppendArgs {
   nsrl_q4_cache c;
   const int16_t* k;
@@ -39,15 +39,16 @@ __device__ __forceinline__ uint4 load8(const int16_t* p, bool vec) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Eight dims to eight codes; scale_word is the group's (LPG lanes of the warp).
-template <int LPG>
-__device__ __forceinline__ uint32_t quantise8(const uint4& u, uint32_t& scale_word) {
+// Sixteen dims to sixteen codes; scale_word is the group's (two lanes of the
+// warp, one where PAIRED is false).
+template <bool PAIRED>
+__device__ __forceinline__ uint2 quantise16(const uint4 (&u)[2], uint32_t& scale_word) {
   // smallest values and smallest complements (so the largest values), two at a time
-  uint32_t low = __vmins2(__vmins2(u.x, u.y), __vmins2(u.z, u.w));
-  uint32_t high = __vmaxs2(__vmaxs2(u.x, u.y), __vmaxs2(u.z, u.w));
+  auto least = [](const uint4& v) { return __vmins2(__vmins2(v.x, v.y), __vmins2(v.z, v.w)); };
+  auto most = [](const uint4& v) { return __vmaxs2(__vmaxs2(v.x, v.y), __vmaxs2(v.z, v.w)); };
+  const uint32_t low = __vmins2(least(u[0]), least(u[1])), high = __vmaxs2(most(u[0]), most(u[1]));
   uint32_t both = __vmins2(__byte_perm(low, ~high, 0x5410), __byte_perm(low, ~high, 0x7632));
-#pragma unroll
-  for (int o = 1; o < LPG; o <<= 1) both = __vmins2(both, __shfl_xor_sync(0xffffffffu, both, o));
+  if (PAIRED) both = __vmins2(both, __shfl_xor_sync(0xffffffffu, both, 1));
   const int lo = (int)(int16_t)(both & 0xFFFF), hi = ~((int)both >> 16);
   const unsigned scale = max(1u, (unsigned)(hi - lo + 14) / 15u);
   // floor(n / d) = n * ceil(2^32 / d) >> 32 while n d < 2^32 (Granlund and
@@ -55,24 +56,29 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& u, uint32_t& scale_wo
   const unsigned d = 2 * scale;
   const unsigned magic = 0xFFFFFFFFu / d + 1;
   const int offset = (int)scale - 2 * lo;
-  const bool top = hi + (int)(scale / 2) > 32767;  // a value may pass 32767
-  int x[8];
-  unpack8(u, x);
-  uint32_t codes = 0;
+  const bool top = hi + (int)(scale / 2) > 32767;  // a value may pass 32767: its code goes one down
+  uint32_t codes[2];
 #pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    int q = (int)__umulhi((unsigned)(2 * x[i] + offset), magic);
-    if (top) q -= lo + (int)scale * q > 32767 ? 1 : 0;
-    codes = codes * 16 + (uint32_t)q;
+  for (int e = 0; e < 2; ++e) {
+    int x[8];
+    unpack8(u[e], x);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) w = w * 16 + __umulhi((unsigned)(2 * x[i] + offset), magic);
+    if (top)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (lo + (int)(scale * ((w >> (4 * i)) & 15)) > 32767) w -= 1u << (4 * i);
+    codes[e] = w;
   }
   scale_word = scale | ((uint32_t)lo << 16);
-  return codes;
+  return make_uint2(codes[0], codes[1]);
 }
 
 template <int HD>
 __global__ void __launch_bounds__(THREADS) q4_append_kernel(const AppendArgs a, const bool vec) {
-  constexpr int LPR = HD / 8;                // lanes of a row
-  constexpr int LPG = HD < 32 ? HD / 8 : 4;  // lanes of a group
+  constexpr int LPR = HD / 16;               // lanes of a row
+  constexpr int LPG = HD < 32 ? 1 : 2;       // lanes of a group
   constexpr int G = HD < 32 ? 1 : HD / 32;
   griddep_wait();
   griddep_launch();
@@ -87,18 +93,21 @@ __global__ void __launch_bounds__(THREADS) q4_append_kernel(const AppendArgs a, 
   if (inside && !fits && t == 0 && sub == 0 && h == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
   const bool live = inside && fits && (long long)t < count;
   if (!__any_sync(0xffffffffu, live)) return;
-  uint4 uk = make_uint4(0, 0, 0, 0), uv = uk;
+  uint4 uk[2] = {}, uv[2] = {};
   if (live) {
-    const long long off = ((long long)b * a.tokens + t) * a.ld + (long long)h * HD + 8 * sub;
-    uk = load8(a.k + off, vec);
-    uv = load8(a.v + off, vec);
+    const long long off = ((long long)b * a.tokens + t) * a.ld + (long long)h * HD + 16 * sub;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      uk[e] = load8(a.k + off + 8 * e, vec);
+      uv[e] = load8(a.v + off + 8 * e, vec);
+    }
   }
   uint32_t sk, sv;
-  const uint32_t ck = quantise8<LPG>(uk, sk), cv = quantise8<LPG>(uv, sv);
+  const uint2 ck = quantise16<LPG == 2>(uk, sk), cv = quantise16<LPG == 2>(uv, sv);
   if (!live) return;
   const size_t slot = (size_t)bh * a.c.capacity + (size_t)(start + t);
-  reinterpret_cast<uint32_t*>(a.c.k_codes)[slot * LPR + sub] = ck;
-  reinterpret_cast<uint32_t*>(a.c.v_codes)[slot * LPR + sub] = cv;
+  reinterpret_cast<uint2*>(a.c.k_codes)[slot * LPR + sub] = ck;
+  reinterpret_cast<uint2*>(a.c.v_codes)[slot * LPR + sub] = cv;
   if (sub % LPG == 0) {
     a.c.k_scales[slot * G + sub / LPG] = sk;
     a.c.v_scales[slot * G + sub / LPG] = sv;
@@ -119,11 +128,6 @@ struct ReadArgs {
   nsrl_device_status* st;
 };
 
-// Rows of a thread, loaded before the first is written: 2,048 rows of 2,048 slots
-// take 245 us one at a time and 218 two or four at a time (99% of copy
-// bandwidth); 2,048 single slots 5.5, 5.5 and 7.
-constexpr int READ_ROWS = 2;
-
 __device__ __forceinline__ uint4 dequantise8(uint32_t codes, uint32_t scale_word) {
   const int scale = (int)(scale_word & 0xFFFF), zero = (int)(int16_t)(scale_word >> 16);
   uint32_t w[4];
@@ -133,43 +137,49 @@ __device__ __forceinline__ uint4 dequantise8(uint32_t codes, uint32_t scale_word
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Read: a lane takes pieces of 8 dims, half a row apart where a row has more than
+// two, so that four accesses are under way and each store of a warp fills whole
+// sectors.  2,048 rows of 2,048 slots take 211 us, all of the copy bandwidth (218
+// with two rows of 8 dims a thread, 245 with one).
+template <int HD>
+struct ReadShape {
+  static constexpr int E = HD == 16 ? 1 : 2;          // pieces of a lane
+  static constexpr int LPR = HD / (8 * E);            // lanes of a row
+  static constexpr int ROWS = THREADS / LPR;          // rows of a block
+};
+
 template <int HD>
 __global__ void __launch_bounds__(THREADS) q4_read_kernel(const ReadArgs a) {
-  constexpr int LPR = HD / 8;
-  constexpr int LPG = HD < 32 ? HD / 8 : 4;
-  constexpr int G = HD < 32 ? 1 : HD / 32;
-  constexpr int U = READ_ROWS, PER = THREADS / LPR;
+  using S = ReadShape<HD>;
+  constexpr int G = HD < 32 ? 1 : HD / 32, PPG = HD < 32 ? HD / 8 : 4;  // groups, pieces of a group
+  constexpr int E = S::E, LPR = S::LPR;
   griddep_wait();
   griddep_launch();
   const int sub = threadIdx.x % LPR;
+  const unsigned row = blockIdx.x * S::ROWS + threadIdx.x / LPR;
+  if (row >= a.rows) return;
   const unsigned tokens = (unsigned)a.tokens;
-  uint32_t ck[U], cv[U], sk[U], sv[U];
-  bool ok[U];
-  const unsigned row0 = blockIdx.x * (PER * U) + threadIdx.x / LPR;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const unsigned row = row0 + u * PER;
-    ok[u] = row < a.rows;
-    if (!ok[u]) continue;
-    const unsigned bh = row / tokens, t = row - bh * tokens, b = bh / (unsigned)a.c.heads;
-    const long long start = a.starts ? (long long)a.starts[b] : 0;
-    if (start < 0 || start + a.tokens > (long long)a.c.capacity) {
-      if (t == 0 && sub == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
-      ok[u] = false;
-      continue;
-    }
-    const size_t slot = (size_t)bh * a.c.capacity + (size_t)(start + t);
-    ck[u] = reinterpret_cast<const uint32_t*>(a.c.k_codes)[slot * LPR + sub];
-    cv[u] = reinterpret_cast<const uint32_t*>(a.c.v_codes)[slot * LPR + sub];
-    sk[u] = a.c.k_scales[slot * G + sub / LPG];
-    sv[u] = a.c.v_scales[slot * G + sub / LPG];
+  const unsigned bh = row / tokens, t = row - bh * tokens, b = bh / (unsigned)a.c.heads;
+  const long long start = a.starts ? (long long)a.starts[b] : 0;
+  if (start < 0 || start + a.tokens > (long long)a.c.capacity) {
+    if (t == 0 && sub == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
+    return;
   }
+  const size_t slot = (size_t)bh * a.c.capacity + (size_t)(start + t);
+  uint32_t ck[E], cv[E], sk[E], sv[E];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (!ok[u]) continue;
-    const size_t i = (size_t)(row0 + u * PER) * LPR + sub;
-    reinterpret_cast<uint4*>(a.k)[i] = dequantise8(ck[u], sk[u]);
-    reinterpret_cast<uint4*>(a.v)[i] = dequantise8(cv[u], sv[u]);
+  for (int e = 0; e < E; ++e) {
+    const int piece = sub + LPR * e;
+    ck[e] = reinterpret_cast<const uint32_t*>(a.c.k_codes)[slot * (HD / 8) + piece];
+    cv[e] = reinterpret_cast<const uint32_t*>(a.c.v_codes)[slot * (HD / 8) + piece];
+    sk[e] = a.c.k_scales[slot * G + piece / PPG];
+    sv[e] = a.c.v_scales[slot * G + piece / PPG];
+  }
+  const size_t i = (size_t)row * (HD / 8) + sub;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    reinterpret_cast<uint4*>(a.k)[i + LPR * e] = dequantise8(ck[e], sk[e]);
+    reinterpret_cast<uint4*>(a.v)[i + LPR * e] = dequantise8(cv[e], sv[e]);
   }
 }
 
@@ -536,7 +546,7 @@ size_t list_offset(const nsrl_q4_cache& c) { return (c.batch * c.heads * sizeof(
 cudaError_t launch_q4_append(const nsrl_q4_cache& c, const int16_t* k, const int16_t* v, size_t ld, size_t tokens,
                              const int32_t* starts, const int32_t* counts, const int32_t* positions,
                              nsrl_device_status* st, cudaStream_t s) {
-  const size_t n = c.batch * c.heads * tokens, per_block = THREADS / (c.head_dim / 8);
+  const size_t n = c.batch * c.heads * tokens, per_block = THREADS / (c.head_dim / 16);
   if (n == 0) return cudaSuccess;
   if (n > 0xffffff00u) return cudaErrorInvalidValue;  // the entry point refuses it
   const AppendArgs a{c, k, v, (long long)ld, (long long)tokens, (unsigned)n, starts, counts, positions, st};
@@ -550,7 +560,10 @@ cudaError_t launch_q4_append(const nsrl_q4_cache& c, const int16_t* k, const int
 
 cudaError_t launch_q4_read(const nsrl_q4_cache& c, const int32_t* starts, size_t tokens, int16_t* k, int16_t* v,
                            nsrl_device_status* st, cudaStream_t s) {
-  const size_t n = c.batch * c.heads * tokens, per_block = READ_ROWS * THREADS / (c.head_dim / 8);
+  const size_t n = c.batch * c.heads * tokens;
+  const size_t per_block = c.head_dim == 16   ? ReadShape<16>::ROWS
+                           : c.head_dim == 64 ? ReadShape<64>::ROWS
+                                              : ReadShape<256>::ROWS;
   if (n == 0) return cudaSuccess;
   if (n > 0xffffff00u) return cudaErrorInvalidValue;  // the entry point refuses it
   const ReadArgs a{c, starts, (long long)tokens, (unsigned)n, k, v, st};
