@@ -121,9 +121,8 @@ class Q4Cache:
         if rows % max(1, self.batch) or k.shape[1] != cols or v.shape[1] != cols:
             raise core.NsrlError("k and v must be [batch * tokens, heads * head_dim]")
         stream = self._stream()
-        kp, vp = core._rows(k, rows, cols, self._dev, "k"), core._rows(v, rows, cols, self._dev, "v")
-        ld = core._row_stride(k)
-        if rows > 1 and v.stride(0) != ld:
+        (kp, ld), (vp, vld) = core._rows(k, rows, cols, self._dev, "k"), core._rows(v, rows, cols, self._dev, "v")
+        if rows > 1 and vld != ld:
             raise core.NsrlError("k and v must have one row stride")
         return _lib().nsrl_q4_cache_append(self._ref, kp, vp, ld, rows // max(1, self.batch),
                                            self._per_sequence(starts, "starts"),
@@ -153,10 +152,10 @@ class Q4Cache:
         wp, wn = self._ws_ptr, self._ws_bytes
         if ws is not None:
             wp, wn = core._array(ws, torch.uint8, ws.shape, self._dev, "the workspace"), ws.numel()
-        qp = core._rows(q, self.batch, cols, self._dev, "q")
+        qp, ldq = core._rows(q, self.batch, cols, self._dev, "q")
         if q.shape[1] != cols:
             raise core.NsrlError("q must be [batch, heads * head_dim]")
-        return _lib().nsrl_attention_decode_q4(qp, core._row_stride(q), self._ref, self._per_sequence(lens, "lens"),
+        return _lib().nsrl_attention_decode_q4(qp, ldq, self._ref, self._per_sequence(lens, "lens"),
                                                core._array(ctx, torch.int16, (self.batch, cols), self._dev, "ctx"),
                                                wp, wn, status.buf.data_ptr(), stream)
 
@@ -225,7 +224,7 @@ def prenorm_attention_decode_block_q4(x, rms_gamma, rms_eps, q, k, v, o, cache: 
         if rotary.turns.get_device() != cache._dev:
             raise core.NsrlError(f"the rotary plan is on {rotary.turns.device}, the cache on {cache.device}")
     stream = cache._stream()
-    xp = core._rows(x, B, d, cache._dev, "x")
+    xp, _ = core._rows(x, B, d, cache._dev, "x")
     lp = cache._per_sequence(lens, "lens")
     pp = None if positions is None else cache._per_sequence(positions, "positions")
     y = torch.empty_like(x)

@@ -193,19 +193,16 @@ def _array(t: torch.Tensor, dtype, shape, device: int, what: str) -> int:
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, rows: int, cols: int, device: int, what: str) -> int:
-    """The address of int16 rows of at least `cols` contiguous columns on the current device."""
+def _rows(t: torch.Tensor, rows: int, cols: int, device: int, what: str):
+    """Address and row stride of int16 rows of at least `cols` contiguous columns on
+    the current device (one row's stride may be anything: its width stands in)."""
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.int16 or t.get_device() != device or t.dim() != 2:
         _refuse(t, torch.int16, device, what, "rows")
     n, width = t.shape
-    if n != rows or width < cols or (width > 1 and t.stride(1) != 1):
+    ld, step = t.stride()
+    if n != rows or width < cols or (width > 1 and step != 1):
         _refuse(t, torch.int16, device, what, f"{rows} rows of at least {cols} contiguous columns")
-    return t.data_ptr()
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Row stride of a 2-D tensor (its width where there is one row, whose stride may be anything)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+    return t.data_ptr(), (ld if n > 1 else max(width, ld))
 
 
 # ----------------------------------------------------------------- linear ---

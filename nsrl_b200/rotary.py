@@ -112,17 +112,17 @@ class Rotary:
         L, dev = _lib(), torch.cuda.current_device()
         cols = heads * self.head_dim
         rows = x.shape[0]
-        xp = core._rows(x, rows, cols, dev, "x")
+        xp, ldx = core._rows(x, rows, cols, dev, "x")
         pp = None if positions is None else core._array(positions, torch.int32, (rows,), dev, "positions")
         if self.turns.get_device() != dev:
             core._refuse(self.turns, torch.int64, dev, "the rotary plan", "on the current device")
         if out is None:
             out = torch.empty((rows, cols), dtype=torch.int16, device=x.device)
-        yp = core._rows(out, rows, cols, dev, "out")
+        yp, ldy = core._rows(out, rows, cols, dev, "out")
         if rows == 0:
             return out
-        r = L.nsrl_rotary_rows(xp, rows, heads, self.head_dim, core._row_stride(x), self._ref, pp, seq_len,
-                               1 if backward else 0, yp, core._row_stride(out), core._raw_stream(dev))
+        r = L.nsrl_rotary_rows(xp, rows, heads, self.head_dim, ldx, self._ref, pp, seq_len,
+                               1 if backward else 0, yp, ldy, core._raw_stream(dev))
         if r == core.NSRL_OK:
             return out
         if r == core.NSRL_INVALID_SHAPE:
