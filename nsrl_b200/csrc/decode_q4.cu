@@ -24,7 +24,8 @@
 // spends less than about 3.5 cycles on a slot, that is some 14 instructions of
 // a warp on 32 slots each cycle it has; the integer pipes take one every other
 // cycle.  So instructions are counted:
-//   keys:   a lane owns a slot and loads its whole row; codes widen to bytes and
+//   keys:   a lane owns a slot and loads its whole row (256 dims: eight lanes
+//           a slot, a group each); codes widen to bytes and
 //           meet the query's high (signed) and low (unsigned) byte planes in
 //           dp4a, 32 a slot.
 //   values: int8 MMAs (m16n8k32): A = 16 dims x 32 slots (transposing matrix
@@ -255,10 +256,63 @@ __device__ __forceinline__ void dots16(const Query<HD>& query, const KeyRow<HD> 
   }
 }
 
+// A unit of 256-dim rows: eight lanes a row, each one group of it, so that a load
+// of the warp takes four whole rows and the query stays in registers.  Step i of a
+// lane is row 4 i + (lane >> 3).  64 rows of 8,192 take 50 us, and 60 with a lane a
+// row; at 64 dims the same with two lanes a row is slower (35.2 for 34.3 us, 256
+// rows of 8,192): its registers pass the 64 that two CTAs of 16 warps leave.
+struct KeyUnit256 {
+  uint4 code[8];
+  uint32_t scale[8];
+
+  template <bool ALL>
+  __device__ __forceinline__ void load(const nsrl_q4_cache& c, size_t slot, int left) {
+    const int lane = threadIdx.x & 31, r = lane >> 3;
+    const uint4* p = reinterpret_cast<const uint4*>(c.k_codes + slot * 128) + lane;
+    const uint32_t* s = c.k_scales + slot * 8 + lane;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool there = ALL || 4 * i + r < left;
+      code[i] = there ? __ldcs(p + 32 * i) : make_uint4(0, 0, 0, 0);
+      scale[i] = there ? __ldcs(s + 32 * i) : 0u;
+    }
+  }
+
+  // 16 q . k of row 4 (lane & 7) + (lane >> 3); q: this lane's group of the query
+  __device__ __forceinline__ long long dot16(const uint4 (&q)[4], int sum16) const {
+    const int g = threadIdx.x & 7;
+    long long v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+      int he = 0, ho = 0, le = 0, lo = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        he = dp4a_us(w[k] & LOW, q[k].x, he);
+        ho = dp4a_us(w[k] & HIGH, q[k].y, ho);
+        le = dp4a_uu(w[k] & LOW, q[k].z, le);
+        lo = dp4a_uu(w[k] & HIGH, q[k].w, lo);
+      }
+      const int dot = (he * 256 + le) * 16 + (ho * 256 + lo);
+      v[i] = (long long)dot * (int)(scale[i] & 0xFFFF) + (long long)sum16 * ((int)scale[i] >> 16);
+    }
+    // the eight lanes' groups add up, and lane g keeps step g
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < o; ++i) {
+        const bool upper = g & o;
+        const long long give = upper ? v[i] : v[i + o];
+        v[i] = (upper ? v[i + o] : v[i]) + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    return v[0];
+  }
+};
+
 // Logits of n slots from slot0; returns this warp's maximum (INT_MIN: none
 // counts; MASKED_LOGIT is INT_MIN and never raises it).  A step takes two whole
-// units with the next step's rows under way (one unit and none ahead at 256
-// dims, whose rows fill the registers); what is left over goes unit by unit.
+// units (one at 256 dims) with the next step's rows under way; what is left over
+// goes unit by unit.
 // `ready` is called once, after the first loads and before the query is read.
 template <int HD, int WARPS, typename Ready>
 __device__ __forceinline__ int keys_pass(const AttendArgs& a, const Query<HD>& query, size_t slot0, int n,
@@ -298,17 +352,34 @@ __device__ __forceinline__ int keys_pass(const AttendArgs& a, const Query<HD>& q
       put(at, v[0]);
       put(at + WARPS * UNIT, v[1]);
     }
+    for (; u * UNIT < n; u += WARPS) {
+      const int j = u * UNIT + lane;
+      if (j >= n) continue;
+      KeyRow<HD> row[1];
+      row[0].load(a.c, slot0 + j);
+      long long v[1];
+      dots16<HD, 1>(query, row, v);
+      put(j, v[0]);
+    }
   } else {
+    KeyUnit256 unit, next;
+    if (u < whole) next.load<true>(a.c, slot0 + u * UNIT, UNIT);
     ready();
-  }
-  for (; u * UNIT < n; u += WARPS) {
-    const int j = u * UNIT + lane;
-    if (j >= n) continue;
-    KeyRow<HD> row[1];
-    row[0].load(a.c, slot0 + j);
-    long long v[1];
-    dots16<HD, 1>(query, row, v);
-    put(j, v[0]);
+    const int g = lane & 7, mine = 4 * g + (lane >> 3);
+    const uint4 q[4] = {query.word[4 * g], query.word[4 * g + 1], query.word[4 * g + 2], query.word[4 * g + 3]};
+    const int sum16 = query.sum16[g];
+    while (u < whole) {
+      unit = next;
+      const int at = u * UNIT + mine;
+      u += WARPS;
+      if (u < whole) next.load<true>(a.c, slot0 + u * UNIT, UNIT);
+      put(at, unit.dot16(q, sum16));
+    }
+    if (u == whole && n % UNIT != 0) {
+      unit.load<false>(a.c, slot0 + u * UNIT, n % UNIT);
+      const long long v = unit.dot16(q, sum16);
+      if (mine < n % UNIT) put(u * UNIT + mine, v);
+    }
   }
   if (bad) nsrl_flag(a.st, NSRL_FLAG_LOGIT_RANGE);
   return __reduce_max_sync(0xffffffffu, mx);
