@@ -206,9 +206,10 @@ def test_attend_long_streams_split(K):
         assert np.array_equal(host(cache.scores), scores)
 
 
-@pytest.mark.parametrize("B,cap", [(150, 32768), (19, 262144)])  # one CTA a row, and eight
+@pytest.mark.parametrize("B,cap", [(150, 32768), (19, 262144), (600, 32784)])
 def test_attend_largest_shares(K, B, cap):
-    """32,768 slots a CTA: the most logits that one keeps."""
+    """32,768 slots a CTA, the most logits that one keeps: one CTA a row, and eight;
+    and rows sorted by length of two CTAs each."""
     g = torch.Generator(device="cuda").manual_seed(cap)
     draw = lambda lo, hi, shape, t: torch.randint(lo, hi, shape, generator=g, device="cuda").to(t)  # noqa: E731
     kc, vc = (draw(0, 256, (B, 1, cap, 8), torch.uint8) for _ in "kv")
