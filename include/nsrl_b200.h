@@ -287,7 +287,12 @@ nsrl_status nsrl_q4_cache_read(const nsrl_q4_cache* cache, const int32_t* starts
  * int16 ones; the same logits, base-2 softmax and rounding, so on equal values
  * the same context.  ctx: [batch][heads * head_dim].  With
  * cache->scores, the Q15 weight of each slot is added to its score
- * (saturating at 2^31 - 1).  Capacity at most nsrl_q4_cache_max_capacity().
+ * (saturating at 2^31 - 1), unless one of the lens is bad or the status
+ * already holds a rejection (of an earlier call, not reset; a logit's aside):
+ * then every score stays as it was, so that a rejected call may be made again.
+ * Logits outside 32 bits or masked throughout a row show only on the way:
+ * after a rejection for them other rows may have gained their weights.
+ * Capacity at most nsrl_q4_cache_max_capacity().
  * workspace: nsrl_attention_decode_q4_workspace_size(cache) bytes (0 for a
  * small cache: NULL is fine then), 256-byte aligned, its contents of no
  * account before and after; calls that may run at the same time, two captured
@@ -321,7 +326,10 @@ nsrl_status nsrl_q4_cache_evict(const nsrl_q4_cache* cache, const int32_t* lens,
  * and projected, its q and k turn by positions[b] (device int32; NULL =
  * lens[b]), its k and v enter slot lens[b] (device int32, 0..capacity - 1),
  * and its query attends over slots 0 .. lens[b].  The caller advances lens
- * (and positions) after every layer of the step, and evicts between steps. */
+ * (and positions) after every layer of the step, and evicts between steps.  A
+ * call rejected for a full sequence, its norm or its projections leaves slots
+ * 0 .. lens[b] - 1 and their scores as they were (slot lens[b] is unspecified):
+ * it may be made again once the cause is mended. */
 size_t nsrl_decode_block_q4_workspace_size(const nsrl_q4_cache* cache);
 nsrl_status nsrl_prenorm_attention_decode_block_q4(const int16_t* x, size_t batch, size_t d_model, size_t heads,
                                                    const int16_t* rms_gamma, uint64_t rms_eps,

@@ -10,6 +10,11 @@ without waiting (they may be captured into a graph; the device status tells
 rejections later).  The methods without the prefix wait and return None when
 the call was rejected, as the functions of `core` do.
 
+Scores go on from step to step.  A call that is rejected for a length, or whose
+status already holds a rejection, leaves all of them as they were, so a step
+with a full sequence can be made again after an eviction; reset a status that
+`launch_*` calls share after a rejection.
+
 Calls on one cache run one after another: on one stream, or on several that the
 caller orders.  Attention without scores only reads the cache, so it may run on
 several streams at once, each call with a workspace of its own.

@@ -19,6 +19,11 @@
 //           adds them up (integers: in any order the same).  No CTA waits for
 //           another, and chunks spread evenly over the SMs.
 // plan_of() chooses, by sizes alone.
+// Scores go on from call to call, so a call with a bad length, or whose status
+// already holds a rejection, leaves all of them: it can be mended and made again.
+// Bad lengths are known before the first score changes: every CTA looks at all of
+// them (fewer than SORT_ROWS, so at most three a thread), or an earlier launch of
+// the call has.
 //
 // Bound by memory (80 bytes a slot of 64 dims, 88 with scores) while an SM
 // spends less than about 3.5 cycles on a slot, that is some 14 instructions of
@@ -67,6 +72,10 @@ struct Q4Shape {
   static constexpr int SHIFT = HD == 16 ? 2 : HD == 64 ? 3 : 4;
 };
 
+// Flags that a CTA of the running launch may set at any moment: not asked for, so
+// that what a call does to the scores does not depend on the order of its CTAs.
+constexpr unsigned long long FOUND_LATE = NSRL_FLAG_LOGIT_RANGE | NSRL_FLAG_ALL_MASKED;
+
 struct AttendArgs {
   nsrl_q4_cache c;
   const int16_t* q;
@@ -78,6 +87,7 @@ struct AttendArgs {
   // WHOLE's scratch
   int2* order;       // [batch]: (sequence, length), the longest first; NULL: as they come
   int length_shift;  // class of a length
+  bool lens_known;   // an earlier launch has flagged the bad lengths
   // the split form's scratch
   int chunks;           // of a row of `capacity` slots
   int32_t* logits;      // [batch * heads][capacity]
@@ -86,6 +96,14 @@ struct AttendArgs {
   unsigned* arrived;    // [batch * heads]: chunks whose context is written
   long long* partial;   // [batch * heads][chunks][head_dim]
 };
+
+__device__ __forceinline__ unsigned long long flags_of(const AttendArgs& a) {
+  return *reinterpret_cast<const volatile unsigned long long*>(&a.st->flags);
+}
+
+__device__ __forceinline__ bool bad_length(const AttendArgs& a, long long len) {
+  return len <= 0 || len > (long long)a.c.capacity;
+}
 
 __device__ __forceinline__ int dp4a_us(uint32_t a, uint32_t b, int c) {  // unsigned x signed bytes
   int d;
@@ -588,7 +606,11 @@ __global__ void __launch_bounds__(1024) q4_order_kernel(const AttendArgs a) {
   __syncthreads();
   auto length = [&](int i) { return (int)min((long long)a.lens[i] + a.len_offset, (long long)INT_MAX); };
   auto length_class = [&](int len) { return min(max(len, 0) >> a.length_shift, LENGTHS - 1); };
-  for (int i = tid; i < batch; i += 1024) atomicAdd(&count[length_class(length(i))], 1);
+  for (int i = tid; i < batch; i += 1024) {
+    const int len = length(i);
+    if (bad_length(a, len)) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
+    atomicAdd(&count[length_class(len)], 1);
+  }
   __syncthreads();
   if (tid < LENGTHS) {
     int longer = 0;
@@ -600,6 +622,16 @@ __global__ void __launch_bounds__(1024) q4_order_kernel(const AttendArgs a) {
     const int len = length(i);
     a.order[atomicAdd(&next[length_class(len)], 1)] = make_int2(i, len);
   }
+}
+
+// Flags the bad lengths before the attention begins, where a CTA would have too
+// many of them to look through.
+__global__ void __launch_bounds__(256) q4_screen_kernel(const AttendArgs a) {
+  griddep_wait();
+  griddep_launch();
+  const unsigned b = blockIdx.x * 256 + threadIdx.x;
+  if (b < (unsigned)a.c.batch && bad_length(a, (long long)a.lens[b] + a.len_offset))
+    nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
 }
 
 template <int HD, int WARPS>
@@ -615,11 +647,13 @@ __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARP
   __shared__ unsigned s_red[WARPS];
   __shared__ unsigned long long s_sum[MAX_CLUSTER];
   __shared__ long long s_part[WARPS / S::PAIRS][HD], s_ctx[HD];
+  __shared__ int s_hold;  // the scores stay as they are
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < 256) lut[tid] = d_exp2_lut[tid];
   if (tid < 128) recip[tid] = d_recip_lut[tid];
+  if (tid == 0) s_hold = 0;
   griddep_wait();
   griddep_launch();
   unsigned bh = blockIdx.x / (unsigned)parts, b = bh / (unsigned)a.c.heads;
@@ -634,7 +668,13 @@ __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARP
     len = (long long)a.lens[b] + a.len_offset;
   }
   if (warp == 0) lay_out<HD>(query, a.q + b * a.ldq + (long long)h * HD);
-  if (len <= 0 || len > (long long)a.c.capacity) {  // the same for the whole cluster
+  // The last thread asks for the flags, the others for a length each; they are
+  // looked at once the first keys are on their way.  Waiting ahead of the keys cost
+  // 5 to 13% of a call, waiting after them 2 to 8%, here 0.2 to 0.4 us in one wave.
+  const bool look = a.c.scores && (tid == THREADS - 1 || (!a.lens_known && tid < (int)a.c.batch));
+  int said = 0;
+  if (look) said = tid == THREADS - 1 ? *reinterpret_cast<const int*>(&a.st->flags) : a.lens[tid];
+  if (bad_length(a, len)) {  // the same for the whole cluster
     if (tid == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
     return;
   }
@@ -647,6 +687,13 @@ __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARP
       cluster.sync();  // every CTA has started: its shared memory may be written
     else
       __syncthreads();
+    if (look) {
+      bool hold = tid == THREADS - 1 ? (said & ~(int)FOUND_LATE) != 0 : bad_length(a, (long long)said + a.len_offset);
+      if (!a.lens_known)
+        for (unsigned i = tid + THREADS - 1; i < (unsigned)a.c.batch; i += THREADS - 1)
+          hold |= bad_length(a, (long long)a.lens[i] + a.len_offset);
+      if (hold) s_hold = 1;
+    }
   });
   const ValuePlaces<HD, false> at(a, slot0, logits);
   ValueUnit<HD> next;
@@ -673,7 +720,13 @@ __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARP
     for (int r = 0; r < parts; ++r) sum += s_sum[r];
   }
   const unsigned inv = mx == INT_MIN ? 0u : reciprocal(recip, sum);
-  values_pass<HD, WARPS>(at, next, n, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
+  if (s_hold) {  // its own copy of the pass: a pointer that may be NULL late costs the other 6% in registers
+    ValuePlaces<HD, false> still = at;
+    still.score = nullptr;
+    values_pass<HD, WARPS>(still, next, n, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
+  } else {
+    values_pass<HD, WARPS>(at, next, n, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
+  }
   __syncthreads();
   long long total = 0;
   if (tid < HD) {
@@ -707,7 +760,7 @@ struct Chunk {
     b = bh / (unsigned)a.c.heads;
     h = bh - b * (unsigned)a.c.heads;
     len = (long long)a.lens[b] + a.len_offset;
-    if (len <= 0 || len > (long long)a.c.capacity) return false;
+    if (bad_length(a, len)) return false;
     const long long first = (long long)blockIdx.y * CHUNK;
     if (first >= len) return false;
     n = (int)min((long long)CHUNK, len - first);
@@ -781,9 +834,10 @@ __global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_values_ke
   griddep_launch();
   Chunk c;
   if (!c.find(a)) return;
-  const ValuePlaces<HD, true> at(a, c.slot0, a.logits + c.slot0);
+  ValuePlaces<HD, true> at(a, c.slot0, a.logits + c.slot0);
   ValueUnit<HD> next;
   first_values<HD, SPLIT_WARPS>(at, c.n, next);
+  const unsigned long long flags = flags_of(a);  // the launches before this one have set all there is to set
   // every warp adds up the row's chunks for itself
   int mx = INT_MIN;
   unsigned long long sum = 0;
@@ -794,6 +848,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_values_ke
   mx = __reduce_max_sync(0xffffffffu, mx);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (flags != 0) at.score = nullptr;
   __syncthreads();
   const unsigned inv = mx == INT_MIN ? 0u : reciprocal(recip, sum);
   values_pass<HD, SPLIT_WARPS>(at, next, c.n, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
@@ -951,7 +1006,11 @@ cudaError_t launch_attend_q4(const int16_t* q, size_t ldq, const nsrl_q4_cache& 
       while (c.capacity >> a.length_shift >= LENGTHS) ++a.length_shift;
       e = launch_pdl(q4_order_kernel, dim3(1), dim3(1024), 0, s, a);
       if (e != cudaSuccess) return e;
+    } else if (c.scores && c.batch > SORT_BATCH) {
+      e = launch_pdl(q4_screen_kernel, dim3((unsigned)((c.batch + 255) / 256)), dim3(256), 0, s, a);
+      if (e != cudaSuccess) return e;
     }
+    a.lens_known = p.sorted || c.batch > SORT_BATCH;
     e = c.head_dim == 16   ? (few ? launch_whole<16, 8>(a, p.parts, share, s) : launch_whole<16, 16>(a, p.parts, share, s))
         : c.head_dim == 64 ? (few ? launch_whole<64, 8>(a, p.parts, share, s) : launch_whole<64, 16>(a, p.parts, share, s))
                            : (few ? launch_whole<256, 8>(a, p.parts, share, s) : launch_whole<256, 16>(a, p.parts, share, s));
