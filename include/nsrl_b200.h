@@ -290,8 +290,8 @@ nsrl_status nsrl_q4_cache_read(const nsrl_q4_cache* cache, const int32_t* starts
  * (saturating at 2^31 - 1), unless one of the lens is bad or the status
  * already holds a rejection (of an earlier call, not reset; a logit's aside):
  * then every score stays as it was, so that a rejected call may be made again.
- * Logits outside 32 bits or masked throughout a row show only on the way:
- * after a rejection for them other rows may have gained their weights.
+ * Logits outside 32 bits or masked throughout a row show only on the way: the
+ * rows that have them leave their scores, others may have gained their weights.
  * Capacity at most nsrl_q4_cache_max_capacity().
  * workspace: nsrl_attention_decode_q4_workspace_size(cache) bytes (0 for a
  * small cache: NULL is fine then), 256-byte aligned, its contents of no

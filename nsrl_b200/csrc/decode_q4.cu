@@ -23,7 +23,7 @@
 // already holds a rejection, leaves all of them: it can be mended and made again.
 // Bad lengths are known before the first score changes: every CTA looks at all of
 // them (fewer than SORT_ROWS, so at most three a thread), or an earlier launch of
-// the call has.
+// the call has.  A row with a logit outside 32 bits leaves its own.
 //
 // Bound by memory (80 bytes a slot of 64 dims, 88 with scores) while an SM
 // spends less than about 3.5 cycles on a slot, that is some 14 instructions of
@@ -331,10 +331,11 @@ struct KeyUnit256 {
 // counts; MASKED_LOGIT is INT_MIN and never raises it).  A step takes two whole
 // units (one at 256 dims) with the next step's rows under way; what is left over
 // goes unit by unit.
-// `ready` is called once, after the first loads and before the query is read.
-template <int HD, int WARPS, typename Ready>
+// `ready` is called once, after the first loads and before the query is read,
+// `outside` by a lane that had a logit outside 32 bits.
+template <int HD, int WARPS, typename Ready, typename Outside>
 __device__ __forceinline__ int keys_pass(const AttendArgs& a, const Query<HD>& query, size_t slot0, int n,
-                                         int32_t* logits, Ready ready) {
+                                         int32_t* logits, Ready ready, Outside outside) {
   using S = Q4Shape<HD>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int mx = INT_MIN;
@@ -399,7 +400,10 @@ __device__ __forceinline__ int keys_pass(const AttendArgs& a, const Query<HD>& q
       if (mine < n % UNIT) put(u * UNIT + mine, v);
     }
   }
-  if (bad) nsrl_flag(a.st, NSRL_FLAG_LOGIT_RANGE);
+  if (bad) {
+    nsrl_flag(a.st, NSRL_FLAG_LOGIT_RANGE);
+    outside();
+  }
   return __reduce_max_sync(0xffffffffu, mx);
 }
 
@@ -694,7 +698,7 @@ __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARP
           hold |= bad_length(a, (long long)a.lens[i] + a.len_offset);
       if (hold) s_hold = 1;
     }
-  });
+  }, [&] { s_hold = 1; });  // the weights of this row are of no use
   const ValuePlaces<HD, false> at(a, slot0, logits);
   ValueUnit<HD> next;
   first_values<HD, WARPS>(at, n, next);  // under way while the softmax is worked out
@@ -714,13 +718,17 @@ __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARP
   unsigned long long sum = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) sum += s_red[w];
+  bool hold = s_hold != 0;
   if (parts > 1) {
-    share_out(cluster, s_sum, sum, part, parts);
+    constexpr unsigned long long HELD = 1ull << 40;  // above any sum: 2^30 a CTA
+    share_out(cluster, s_sum, sum + (hold ? HELD : 0), part, parts);
     sum = 0;
     for (int r = 0; r < parts; ++r) sum += s_sum[r];
+    hold = sum >= HELD;
+    sum &= HELD - 1;
   }
   const unsigned inv = mx == INT_MIN ? 0u : reciprocal(recip, sum);
-  if (s_hold) {  // its own copy of the pass: a pointer that may be NULL late costs the other 6% in registers
+  if (hold) {  // its own copy of the pass: a pointer that may be NULL late costs the other 6% in registers
     ValuePlaces<HD, false> still = at;
     still.score = nullptr;
     values_pass<HD, WARPS>(still, next, n, lut, mx, inv, buffer[warp], s_part[warp / S::PAIRS]);
@@ -783,7 +791,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, HD == 256 ? 2 : 4) q4_keys_kern
     if (blockIdx.y == 0 && threadIdx.x == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);  // chunk 0 has slots otherwise
     return;
   }
-  const int mx = keys_pass<HD, SPLIT_WARPS>(a, query, c.slot0, c.n, a.logits + c.slot0, [] { __syncthreads(); });
+  const int mx = keys_pass<HD, SPLIT_WARPS>(a, query, c.slot0, c.n, a.logits + c.slot0, [] { __syncthreads(); }, [] {});
   if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
   __syncthreads();
   if (threadIdx.x == 0) {

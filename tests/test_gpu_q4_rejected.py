@@ -58,6 +58,24 @@ def test_a_status_that_holds_a_rejection(K, form):
     assert torch.equal(ctx, other.attend(q, good)) and torch.equal(cache.scores, other.scores)
 
 
+# (head_dim, capacity, length, the slot): one CTA a row, clusters (the slot in the last CTA's share), the split form
+@pytest.mark.parametrize("hd,cap,n,slot", [(16, 64, 50, 3), (64, 64, 64, 63), (256, 64, 33, 0), (16, 8208, 8200, 8199),
+                                           (64, 8208, 8208, 8207), (256, 2064, 2050, 2049), (64, 32784, 32784, 5),
+                                           (256, 32784, 32784, 32783)])
+def test_a_logit_outside_i32_leaves_its_row(K, hd, cap, n, slot):
+    """One key of 32767s meets a query of 32767s: hd 2^30 >> log4(hd) is 2^32 and more.  The other keys are
+    below 2^9, so their logits fit."""
+    rng = np.random.default_rng(hd + cap)
+    cache, _, _ = filled(K, rng, 2, 1, hd, cap)
+    cache.k_codes[0, 0, slot] = 255
+    cache.k_scales[0, 0, slot] = 1 | (32752 << 16)
+    q = gaussian(rng, (2, hd), 32)
+    q[0] = 32767
+    before = cache.scores.clone()
+    assert cache.attend(dev(q), i32([n, n])) is None
+    assert torch.equal(cache.scores[0], before[0])
+
+
 def linears(d):
     from nsrl_b200 import core, synth as Y
     return [core.Linear(torch.from_numpy(Y.i8_uniform(40 + i, (d, d))), core.make_scales(1, Y.shift_for(d) + up, d))
