@@ -17,7 +17,8 @@ with a full sequence can be made again after an eviction; reset a status that
 
 Calls on one cache run one after another: on one stream, or on several that the
 caller orders.  Attention without scores only reads the cache, so it may run on
-several streams at once, each call with a workspace of its own.
+several streams at once, each call with a workspace of its own: `attend` takes
+one for each call, `launch_attend` takes the cache's unless it is given another.
 """
 from __future__ import annotations
 
@@ -196,8 +197,9 @@ class Q4Cache:
     def attend(self, q, lens) -> Optional[torch.Tensor]:
         """The context rows [batch, heads * head_dim] of q over the first lens[b] slots, or None."""
         ctx = torch.empty((self.batch, self.heads * self.head_dim), dtype=torch.int16, device=self.device)
+        ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device) if self._ws_bytes else None
         st = core.Status()
-        h = core._run(lambda: self.launch_attend(q, lens, ctx, st), st)
+        h = core._run(lambda: self.launch_attend(q, lens, ctx, st, ws), st)
         return None if h is None else ctx
 
     def evict(self, lens, next_positions, keep: int, sinks: int = 4, recent: int = 0) -> Optional[bool]:
