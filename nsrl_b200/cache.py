@@ -235,7 +235,8 @@ def prenorm_attention_decode_block_q4(x, rms_gamma, rms_eps, q, k, v, o, cache: 
     lp = cache._per_sequence(lens, "lens")
     pp = None if positions is None else cache._per_sequence(positions, "positions")
     y = torch.empty_like(x)
-    ws = core.workspace(L.nsrl_decode_block_q4_workspace_size(cache._ref))
+    # of its own, so that blocks on two caches may run at once
+    ws = torch.empty(max(256, L.nsrl_decode_block_q4_workspace_size(cache._ref)), dtype=torch.uint8, device=cache.device)
     st = core.Status()
     ps = [l.c() for l in (q, k, v, o)]
     h = core._run(lambda: L.nsrl_prenorm_attention_decode_block_q4(
