@@ -114,6 +114,12 @@ class Q4Cache:
     def _per_sequence(self, t: torch.Tensor, what: str) -> int:
         return core._array(t, torch.int32, (self.batch,), self._dev, what)
 
+    def _here(self, t: torch.Tensor, what: str) -> int:
+        """The address of a tensor that has its type and shape checked elsewhere, on the cache's device."""
+        if t.get_device() != self._dev:
+            raise core.NsrlError(f"{what} is on {t.device}, the cache on {self.device}")
+        return t.data_ptr()
+
     def _stream(self) -> int:
         if torch.cuda.current_device() != self._dev:
             raise core.NsrlError(f"the cache is on {self.device}, not on the current device")
@@ -134,7 +140,7 @@ class Q4Cache:
                                            self._per_sequence(starts, "starts"),
                                            None if counts is None else self._per_sequence(counts, "counts"),
                                            None if positions is None else self._per_sequence(positions, "positions"),
-                                           status.buf.data_ptr(), stream)
+                                           self._here(status.buf, "the status"), stream)
 
     def launch_read(self, starts, k, v, status: core.Status) -> int:
         """k, v: int16 [batch, heads, tokens, head_dim], written (nsrl_q4_cache_read)."""
@@ -144,8 +150,8 @@ class Q4Cache:
         shape = (self.batch, self.heads, tokens, self.head_dim)
         return _lib().nsrl_q4_cache_read(self._ref, None if starts is None else self._per_sequence(starts, "starts"),
                                          tokens, core._array(k, torch.int16, shape, self._dev, "k"),
-                                         core._array(v, torch.int16, shape, self._dev, "v"), status.buf.data_ptr(),
-                                         stream)
+                                         core._array(v, torch.int16, shape, self._dev, "v"),
+                                         self._here(status.buf, "the status"), stream)
 
     def attend_workspace_bytes(self) -> int:
         return self._ws_bytes
@@ -163,7 +169,7 @@ class Q4Cache:
             raise core.NsrlError("q must be [batch, heads * head_dim]")
         return _lib().nsrl_attention_decode_q4(qp, ldq, self._ref, self._per_sequence(lens, "lens"),
                                                core._array(ctx, torch.int16, (self.batch, cols), self._dev, "ctx"),
-                                               wp, wn, status.buf.data_ptr(), stream)
+                                               wp, wn, self._here(status.buf, "the status"), stream)
 
     def evict_workspace_bytes(self, keep: int) -> int:
         return _lib().nsrl_q4_cache_evict_workspace_size(self._ref, keep)
@@ -177,7 +183,7 @@ class Q4Cache:
             sinks, recent, core._array(scores_out, torch.int32, shape, self._dev, "scores_out"),
             core._array(positions_out, torch.int32, shape, self._dev, "positions_out"),
             self._per_sequence(lens_out, "lens_out"), core._array(ws, torch.uint8, ws.shape, self._dev, "the workspace"),
-            ws.numel(), status.buf.data_ptr(), stream)
+            ws.numel(), self._here(status.buf, "the status"), stream)
 
     # ---- checked calls
     def append(self, k, v, starts, counts=None, positions=None) -> Optional[bool]:
@@ -231,7 +237,11 @@ def prenorm_attention_decode_block_q4(x, rms_gamma, rms_eps, q, k, v, o, cache: 
         if rotary.turns.get_device() != cache._dev:
             raise core.NsrlError(f"the rotary plan is on {rotary.turns.device}, the cache on {cache.device}")
     stream = cache._stream()
+    for name, lin in zip("qkvo", (q, k, v, o)):
+        for t in (lin.weights, lin.scales) + (() if lin.bias is None else (lin.bias,)):
+            cache._here(t, f"the {name} projection")
     xp, _ = core._rows(x, B, d, cache._dev, "x")
+    gp = cache._here(g, "rms_gamma")
     lp = cache._per_sequence(lens, "lens")
     pp = None if positions is None else cache._per_sequence(positions, "positions")
     y = torch.empty_like(x)
@@ -240,7 +250,7 @@ def prenorm_attention_decode_block_q4(x, rms_gamma, rms_eps, q, k, v, o, cache: 
     st = core.Status()
     ps = [l.c() for l in (q, k, v, o)]
     h = core._run(lambda: L.nsrl_prenorm_attention_decode_block_q4(
-        xp, B, d, cache.heads, g.data_ptr(), rms_eps, *[C.byref(p) for p in ps],
+        xp, B, d, cache.heads, gp, rms_eps, *[C.byref(p) for p in ps],
         None if rotary is None else C.byref(rotary.c()), cache._ref, lp, pp, y.data_ptr(), ws.data_ptr(), ws.numel(),
         st.buf.data_ptr(), stream), st)
     return None if h is None else (y, h.attention_saturations)
