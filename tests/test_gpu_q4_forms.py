@@ -1,0 +1,76 @@
+"""Attention over the 4-bit cache in each of its forms: CTAs of 8 and of 16 warps
+at every head dim, clusters of both, the largest shares of slots, and the bound
+of the 32-bit accumulators."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import oracle as O
+
+import q4_plain as P
+from test_gpu_q4_cache import K, dev, filled, gaussian, host, i32  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# one CTA of 16 warps a row (more than 2,048 slots, fewer than 888 rows), unsorted and sorted by length
+FORMS = [(150, 1, 256, 2064), (75, 2, 256, 4112), (600, 1, 256, 2064), (600, 1, 64, 2064), (150, 1, 64, 4112)]
+# 8 warps up to 10,240 slots from 888 rows on, 16 past that
+FORMS += [(222, 4, 256, 2064), (222, 4, 64, 2064), (888, 1, 64, 10240), (888, 1, 64, 10256), (888, 1, 256, 4096)]
+# clusters of 2 CTAs of 16 warps, and of 4
+FORMS += [(75, 1, 256, 8192), (80, 1, 64, 16384), (40, 1, 256, 16400), (37, 2, 16, 16400)]
+
+
+def check_form(K, form, scored):
+    """Context and scores of the longest row, the shortest and some between."""
+    B, H, hd, cap = form
+    g = torch.Generator(device="cuda").manual_seed(B + cap)
+    draw = lambda lo, hi, shape, t: torch.randint(lo, hi, shape, generator=g, device="cuda", dtype=torch.int32).to(t)  # noqa: E731
+    groups = max(1, hd // 32)
+    codes = [draw(0, 256, (B, H, cap, hd // 2), torch.uint8) for _ in "kv"]
+    ks = draw(1, 9, (B, H, cap, groups), torch.int32) | (draw(-60, 1, (B, H, cap, groups), torch.int32) << 16)
+    vs = draw(1, 1000, (B, H, cap, groups), torch.int32) | (draw(-9000, 1, (B, H, cap, groups), torch.int32) << 16)
+    old = draw(0, 1 << 20, (B, H, cap), torch.int32)
+    cache = K.Q4Cache.of(*codes, ks, vs, old.clone() if scored else None)
+    lens = np.random.default_rng(cap).integers(1, cap + 1, B)
+    lens[B // 3], lens[B // 2] = cap, 1
+    q = draw(-40, 41, (B, H * hd), torch.int16)
+    ctx = cache.attend(q, i32(lens))
+    for b in sorted({0, B // 3, B // 2, int(lens.argmax()), B - 1, 7}):
+        one = slice(b, b + 1)
+        k, v = (P.dequantise(host(c[one]), host(s[one])) for c, s in zip(codes, (ks, vs)))
+        want, scores = P.attend(host(q[one]).reshape(1, H, hd), k, v, lens[one], host(old[one]))
+        assert np.array_equal(host(ctx[one]), want)
+        if scored:
+            assert np.array_equal(host(cache.scores[one]), scores)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("scored", [True, False])
+def test_forms_equal_the_oracle(K, form, scored):
+    check_form(K, form, scored)
+
+
+@pytest.mark.parametrize("hd,B,cap", [(64, 150, 32768), (256, 150, 32768), (64, 19, 262144), (256, 19, 262144)])
+def test_largest_shares(K, hd, B, cap):
+    """32,768 slots a CTA at 64 and 256 dims: one CTA a row, and eight."""
+    check_form(K, (B, 1, hd, cap), True)
+
+
+@pytest.mark.parametrize("hd", [16, 64, 256])
+@pytest.mark.parametrize("code", [0xFF, 0xF0, 0x0F])
+def test_the_accumulators_bound(K, hd, code):
+    """32,768 equal logits in one CTA: p = 1 each, so p scale = 65535 is 255 in two byte planes of every slot, and
+    the s32 sums reach 255 * 255 a slot, 255 * 255 * 8,192 a warp at 256 dims.  Dims of code 15 saturate upwards
+    (a wrapped sum would not), dims of code 0 come out as the zero point."""
+    B, cap = 150, 32768
+    p = O.attention_row(np.zeros(hd, np.int16), np.zeros((cap, hd), np.int16), np.zeros((cap, hd), np.int16), hd, hd)[2]
+    assert (np.asarray(p) == 1).all()
+    cache = K.Q4Cache(B, 1, hd, cap)
+    cache.k_scales.fill_(1)
+    cache.v_codes.fill_(code)
+    cache.v_scales.fill_(-1 & 0xFFFF | (-1234 << 16))
+    ctx = host(cache.attend(torch.ones((B, hd), dtype=torch.int16, device="cuda"), i32([cap] * B)))
+    for odd, nibble in ((0, code & 15), (1, code >> 4)):
+        want = min(32767, (cap * (-1234 + 65535 * nibble) + (1 << 14)) >> 15)
+        assert (ctx[:, odd::2] == want).all()
+    assert (host(cache.scores) == 1).all()
