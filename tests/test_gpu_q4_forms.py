@@ -1,6 +1,6 @@
 """Attention over the 4-bit cache in each of its forms: CTAs of 8 and of 16 warps
-at every head dim, clusters of both, the largest shares of slots, and the bound
-of the 32-bit accumulators."""
+at every head dim, clusters of both, the largest shares of slots, the bound of
+the 32-bit accumulators, and masked slots next to live ones."""
 import numpy as np
 import pytest
 import torch
@@ -74,3 +74,38 @@ def test_the_accumulators_bound(K, hd, code):
         want = min(32767, (cap * (-1234 + 65535 * nibble) + (1 << 14)) >> 15)
         assert (ctx[:, odd::2] == want).all()
     assert (host(cache.scores) == 1).all()
+
+
+# one launch, clusters, the split form; whole units of 32 slots and what is left over
+@pytest.mark.parametrize("cap", [64, 8208, 262144])
+@pytest.mark.parametrize("n", [16, 13, 64, 33])
+def test_masked_slots_beside_live_ones_near_the_lowest(K, cap, n):
+    """All logits are -2^31 (MASKED_LOGIT: no weight) but two that are 100 and 348 above it, so that -2^31 weighs
+    something unless it is left out: -32768 * 32768 on 16 of 64 dims is -2^34, >> 3; 8 * 100 and 8 * 348 on another."""
+    cache = K.Q4Cache(2, 1, 64, cap)
+    cache.k_scales[..., 0] = 1 | (32767 << 16)  # first group: 32767 + 1
+    cache.k_codes[..., :16] = 0x11
+    cache.k_scales[..., 1] = 100                # second group: 100 times the code
+    rng = np.random.default_rng(n)
+    values = gaussian(rng, (2, n, 64), 4096)
+    codes, words = P.quantise(values)
+    cache.v_codes[:, 0, :n], cache.v_scales[:, 0, :n] = dev(codes), dev(words)
+    values = P.dequantise(codes, words).astype(np.int16)
+    live = [(3, 1), (n - 2, 3)]
+    for slot, code in live:
+        cache.k_codes[:, 0, slot, 16] = code    # dim 32
+    cache.k_scales[:, 0, n - 2, 1] = 116        # 348 = 3 * 116
+    q = torch.zeros((2, 64), dtype=torch.int16, device="cuda")
+    q[:, :16] = -32768
+    q[:, 32] = 8
+    before = host(cache.scores).copy()
+    got = cache.attend(q, i32([n, n]))
+    # the same two slots with logits 0 and -248: weights go by differences
+    query, keys = np.zeros(64, np.int16), np.zeros((2, 64), np.int16)
+    query[0], keys[0, 0] = 8, -248
+    for b in range(2):
+        want = O.attention_row(query, keys, values[b, [3, n - 2]], 64, 64)
+        assert np.array_equal(host(got)[b], want[0])
+        scores = before[b, 0].copy()
+        scores[[3, n - 2]] += np.asarray(want[2]).astype(np.int32)
+        assert want[2][0] > 0 and np.array_equal(host(cache.scores)[b, 0], scores)
