@@ -200,3 +200,21 @@ def test_training_path(R):
     both = torch.cat(list(grads[:2]), 1)
     plan.apply(both, 2 * H, seq_len=S, backward=True, out=both)
     assert np.array_equal(both.cpu().numpy(), want) and np.array_equal(grads[2].cpu().numpy(), dv)
+
+
+# (heads, head_dim, rotary_dim, row stride - heads * head_dim): wide loads, odd strides, part of a head
+@pytest.mark.parametrize("shape", [(3, 64, 64, 8), (3, 64, 32, 0), (2, 64, 48, 5), (3, 10, 6, 1)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("amplitude", [0.7, 1.2079441541679836, 1.9999999995])
+def test_amplitude_in_every_form(R, shape, layout, backward, amplitude):
+    heads, hd, rot, pad = shape
+    cols = heads * hd
+    plan = R.Rotary(hd, rot, 10000, layout, amplitude=amplitude)
+    x = rows_of(hd + pad, 70, cols + pad)
+    pos = np.random.default_rng(pad).integers(-1000, 200000, 70).astype(np.int32)
+    ref = P.rotate(x[:, :cols], heads, hd, turns_of(plan), layout, pos, backward, plan.c().amplitude)
+    xg = dev(x)
+    assert np.array_equal(plan.apply(xg, heads, dev(pos), backward=backward).cpu().numpy(), ref)
+    plan.apply(xg, heads, dev(pos), backward=backward, out=xg)
+    assert np.array_equal(xg.cpu().numpy()[:, :cols], ref) and np.array_equal(xg.cpu().numpy()[:, cols:], x[:, cols:])
