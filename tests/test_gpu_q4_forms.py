@@ -1,6 +1,7 @@
 """Attention over the 4-bit cache in each of its forms: CTAs of 8 and of 16 warps
 at every head dim, clusters of both, the largest shares of slots, the bound of
-the 32-bit accumulators, and masked slots next to live ones."""
+the 32-bit accumulators, masked slots next to live ones, and arrays past 2^32
+bytes."""
 import numpy as np
 import pytest
 import torch
@@ -109,3 +110,36 @@ def test_masked_slots_beside_live_ones_near_the_lowest(K, cap, n):
         scores = before[b, 0].copy()
         scores[[3, n - 2]] += np.asarray(want[2]).astype(np.int32)
         assert want[2][0] > 0 and np.array_equal(host(cache.scores)[b, 0], scores)
+
+
+def test_arrays_past_32_bits(K):
+    """Codes of 4.3 GB each: append, read, attention and eviction at the end of the last row."""
+    B, hd, cap = 129, 256, 262144
+    assert B * cap * hd // 2 > 1 << 32
+    rng = np.random.default_rng(23)
+    cache = K.Q4Cache(B, 1, hd, cap)
+    k, v = gaussian(rng, (2 * B, hd), 300), gaussian(rng, (2 * B, hd), 4096)
+    k[-2] = k[-1]  # the last row's query weighs its two tokens alike, and nothing else
+    starts = [cap - 2] * B
+    assert cache.append(dev(k), dev(v), i32(starts)) is True
+    kq, vq = P.quantise(k.reshape(B, 1, 2, hd)), P.quantise(v.reshape(B, 1, 2, hd))
+    kr, vr = cache.read(2, i32(starts))
+    assert np.array_equal(host(kr), P.dequantise(*kq)) and np.array_equal(host(vr), P.dequantise(*vq))
+    assert torch.equal(cache.k_codes[-1, 0, cap - 2:], dev(kq[0])[-1, 0])
+    assert int(cache.k_codes[1:, :, :cap - 2].amax()) == 0 and int(cache.k_scales[-1, :, :cap - 2].amax()) == 0
+    q = gaussian(rng, (B, hd), 32)
+    q[-1] = k[-1] // 8
+    lens = [2] * (B - 1) + [cap]
+    ctx = host(cache.attend(dev(q), i32(lens)))
+    full = [np.zeros((1, 1, cap, hd), np.int16) for _ in "kv"]
+    for t, new in zip(full, (kq, vq)):
+        t[0, 0, -2:] = P.dequantise(*new)[-1, 0]
+    want, scores = P.attend(q[-1:].reshape(1, 1, hd), *full, [cap], np.zeros((1, 1, cap), np.int32))
+    assert np.array_equal(ctx[-1:], want) and (ctx[:-1] == 0).all()
+    assert np.array_equal(host(cache.scores[-1:]), scores) and scores[0, 0, -2:].min() > 16000
+    cache.scores.zero_()
+    lens = i32([cap] * B)
+    assert cache.evict(lens, lens.clone(), 16, 0, 2) is True and host(lens).tolist() == [16] * B
+    for got, new in ((cache.k_codes, kq[0]), (cache.v_codes, vq[0]), (cache.k_scales, kq[1]), (cache.v_scales, vq[1])):
+        assert torch.equal(got[:, :, 14:16], dev(new)) and int(got[:, :, :14].abs().max() if got.dtype == torch.int32 else got[:, :, :14].max()) == 0
+    assert host(cache.positions[-1, 0, :16]).tolist() == [0] * 14 + [cap - 2, cap - 1]

@@ -218,3 +218,18 @@ def test_amplitude_in_every_form(R, shape, layout, backward, amplitude):
     assert np.array_equal(plan.apply(xg, heads, dev(pos), backward=backward).cpu().numpy(), ref)
     plan.apply(xg, heads, dev(pos), backward=backward, out=xg)
     assert np.array_equal(xg.cpu().numpy()[:, :cols], ref) and np.array_equal(xg.cpu().numpy()[:, cols:], x[:, cols:])
+
+
+@pytest.mark.parametrize("stride", [1100000008, 1100000003])
+def test_rows_past_32_bits(R, stride):
+    """Rows 2.2 GB apart, so the last begins past 2^31 elements and 2^32 bytes; in place, and out of it."""
+    plan = R.Rotary(64)
+    x = rows_of(13, 3, 128)
+    pos = np.array([5, -7, 123456], np.int32)
+    ref = P.rotate(x, 2, 64, turns_of(plan), "half", pos)
+    far = torch.empty(2 * stride + 128, dtype=torch.int16, device="cuda").as_strided((3, 128), (stride, 1))
+    assert 2 * stride > 1 << 31
+    far.copy_(dev(x))
+    assert np.array_equal(plan.apply(far, 2, dev(pos)).cpu().numpy(), ref)
+    plan.apply(far, 2, dev(pos), out=far)
+    assert np.array_equal(far.cpu().numpy(), ref)
