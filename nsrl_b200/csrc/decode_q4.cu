@@ -153,8 +153,9 @@ __device__ __forceinline__ unsigned weight(const int16_t* lut, int lg, int mx) {
 }
 
 // recip_sum_q31 with the table in shared memory.  Where any logit counts, the
-// slot at the maximum weighs 32767, so the sum is at least that (it is smaller
-// only after a timeout), the result at most 65793.
+// slot at the maximum weighs 32767, so the sum is at least that, the result at most
+// 65793.  A smaller one can only come from a workspace that another call writes to
+// at the same time: a wrong answer then, but no access outside the table.
 __device__ __forceinline__ unsigned reciprocal(const uint32_t* recip, unsigned long long sum) {
   if (sum < 32767) return 0;
   const int shift = 63 - __clzll((long long)sum) - 7;
@@ -278,7 +279,8 @@ __device__ __forceinline__ void dots16(const Query<HD>& query, const KeyRow<HD> 
 // of the warp takes four whole rows and the query stays in registers.  Step i of a
 // lane is row 4 i + (lane >> 3).  64 rows of 8,192 take 50 us, and 60 with a lane a
 // row; at 64 dims the same with two lanes a row is slower (35.2 for 34.3 us, 256
-// rows of 8,192): its registers pass the 64 that two CTAs of 16 warps leave.
+// rows of 8,192): its registers pass the 64 that two CTAs of 16 warps leave
+// (the kept form is at that limit itself and spills 76 bytes).
 struct KeyUnit256 {
   uint4 code[8];
   uint32_t scale[8];
@@ -944,6 +946,13 @@ struct Q4Plan {
 // us, 1,280 80 and 97, 2,048 of 8,320 127 and 144; equal lengths: 90.6 and
 // 88.5, 234 and 232; 8,192 rows of 128 slots 66.9 and 64.0.  Past SORT_BATCH
 // sequences waves are so many that their end counts for little.
+//
+// Where no head dim is named these are rows of 64 dims, and the limits hold for all:
+// at 256 dims an SM has half as many CTAs, so the same numbers of rows are twice as
+// many waves there (not measured apart).
+//
+// Lengths are not seen here: a row takes the form, the CTAs and the shared memory
+// of its capacity, however few of its slots are in use.
 Q4Plan plan_of(const nsrl_q4_cache& c) {
   Q4Plan p{};
   const size_t bh = c.batch * c.heads;

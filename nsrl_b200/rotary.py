@@ -1,9 +1,10 @@
 """Rotary positions on int16 query and key rows (nsrl_rotary_rows).
 
-The reference's models learn their positions or have none; this is the third
-position policy a model of this package can have: the queries and keys of a
-Q|K|V projection turn before the attention (`apply` on the q | k columns), and
-the gradients of the attention backward turn back (`backward=True`).
+The reference's models learn their positions or have none.  Here the queries and
+keys of a Q|K|V projection turn before an attention called by itself (`apply` on
+the q | k columns), and the gradients of its backward turn back
+(`backward=True`); `cache.prenorm_attention_decode_block_q4` takes a plan.  The
+fused transformer block, `train.TrainModel` and the generators take none.
 
 The angles are 64-bit fractions of a turn, so positions far into a long
 context lose nothing, and cos and sin are integer functions of them (the
