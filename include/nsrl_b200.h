@@ -327,9 +327,10 @@ nsrl_status nsrl_q4_cache_evict(const nsrl_q4_cache* cache, const int32_t* lens,
  * lens[b]), its k and v enter slot lens[b] (device int32, 0..capacity - 1),
  * and its query attends over slots 0 .. lens[b].  The caller advances lens
  * (and positions) after every layer of the step, and evicts between steps.  A
- * call rejected for a full sequence, its norm or its projections leaves slots
- * 0 .. lens[b] - 1 and their scores as they were (slot lens[b] is unspecified):
- * it may be made again once the cause is mended. */
+ * call rejected for a full sequence, its norm or its q, k or v projection leaves
+ * slots 0 .. lens[b] - 1 and their scores as they were (slot lens[b] is
+ * unspecified): it may be made again once the cause is mended.  Rejections found
+ * later, in the logits or the output projection, come after scores have changed. */
 size_t nsrl_decode_block_q4_workspace_size(const nsrl_q4_cache* cache);
 nsrl_status nsrl_prenorm_attention_decode_block_q4(const int16_t* x, size_t batch, size_t d_model, size_t heads,
                                                    const int16_t* rms_gamma, uint64_t rms_eps,

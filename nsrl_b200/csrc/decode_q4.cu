@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(32 * WARPS, HD == 256 ? 16 / WARPS : 32 / WARP
   // 5 to 13% of a call, waiting after them 2 to 8%, here 0.2 to 0.4 us in one wave.
   const bool look = a.c.scores && (tid == THREADS - 1 || (!a.lens_known && tid < (int)a.c.batch));
   int said = 0;
-  if (look) said = tid == THREADS - 1 ? *reinterpret_cast<const int*>(&a.st->flags) : a.lens[tid];
+  if (look) said = tid == THREADS - 1 ? (int)flags_of(a) : a.lens[tid];
   if (bad_length(a, len)) {  // the same for the whole cluster
     if (tid == 0) nsrl_flag(a.st, NSRL_FLAG_BAD_LENGTH);
     return;
